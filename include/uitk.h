@@ -352,6 +352,61 @@ int uitk_general_forward(uitk_general* m, const void* pcm, int in_dtype, int64_t
 /* out [B, n_mels, frames]: what self.front_end(x) returns (models/uit.py:455), the batch-global top_db floor applied */
 int uitk_general_mel_db(uitk_general* m, const void* pcm, int in_dtype, int64_t B, int64_t T, float* out, void* stream);
 
+/* ---- Operators on packed 4-bit matrices (csrc/mx4.hip, mx4_dev.h) and the fused seam between two blocks (csrc/block_norm.hip): what the
+ * general engine's precision UITK_PREC_MX4 is made of, callable by themselves.  Stateless: no model handle; caller-owned device
+ * buffers; enqueue-only on `stream` of the current device, nothing allocated, safe inside a stream capture.  Zero rows: nothing is done.
+ *
+ * MXFP4: 32 consecutive elements of a row share a scale 2^X, X = max(floor(log2 max|v|) - 2, -127); an element is v / 2^X rounded to the nearest of
+ * +-{0, .5, 1, 1.5, 2, 3, 4, 6} (ties to the even code, beyond 6 to 6).  A block that holds an infinity or a NaN is NaN as a whole.
+ * The last block of a row may be short.  Packed matrices are opaque buffers of uitk_mx4_bytes, 16-byte aligned. */
+typedef enum uitk_type { UITK_T_F32 = 0, UITK_T_F16 = 1, UITK_T_BF16 = 2, UITK_T_MX4 = 3 } uitk_type;
+
+/* bytes of a packed matrix (-1: rows or K out of range; rows 0 .. 2^31, K 1 .. 2^20) */
+int64_t uitk_mx4_bytes(int64_t rows, int64_t K);
+/* q = packed x; x [rows, K] of `type` (f32 / f16 / bf16), rows `ld` elements apart */
+int uitk_mx4_quantize(const void* x, int type, int64_t rows, int64_t K, int64_t ld, void* q, void* stream);
+/* x = the values of q, rounded once to `type` (exact for f32 and bf16; f16 has no room for block scales far from 1) */
+int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int type, int64_t ld, void* stream);
+
+/* out[M, N] = residual + act(Q(x) . W^T + bias): Q(x) the 4-bit rounding of x [M, K] (or x packed already: x_type UITK_T_MX4), W packed [N, K].
+ * Products are exact, sums are fp32, the output is rounded once.  out_type UITK_T_MX4: `out` is a packed [M, N] matrix -- the next layer's x. */
+typedef struct uitk_mx4_linear_args {
+    const void* x;         /* [M, K], rows ldx elements apart; or packed */
+    const void* w;         /* packed [N, K] */
+    const float* bias;     /* [N] or NULL */
+    const void* residual;  /* [M, N] of out_type, rows ldr apart, or NULL; may be `out` itself */
+    void* out;             /* [M, N], rows ldo apart; or packed */
+    void* workspace;       /* uitk_mx4_linear_workspace bytes, 16-byte aligned, of this call until it has run (NULL when 0) */
+    int64_t M, N, K, ldx, ldr, ldo;
+    int32_t x_type, out_type; /* uitk_type */
+    int32_t act;           /* 0 none, 1 ReLU, 2 exact (erf) GELU */
+    int32_t reserved;      /* 0 */
+} uitk_mx4_linear_args;
+int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type);   /* bytes; -1: out of range */
+int uitk_mx4_linear(const uitk_mx4_linear_args* a, void* stream);
+
+/* residual_out = residual + gate * scale * post(y);  h = pre(residual_out).  post / pre: LayerNorm or root mean square over D, in fp32; h is taken
+ * from the unrounded sum.  y NULL: h = pre(residual) only (no post, gate, scale; residual_out is not written).
+ * Stands in for the residual adds, LayerScale and norms of Block.forward (models/uit.py:244-247, 78-85). */
+typedef enum uitk_norm { UITK_NORM_LAYER = 0, UITK_NORM_RMS = 1 } uitk_norm;
+typedef struct uitk_block_norm_args {
+    const void* y;                         /* [rows, D] the block's output, or NULL */
+    const void* residual;                  /* [rows, D] */
+    void* residual_out;                    /* [rows, D] of r_type; may be `residual` itself */
+    void* h;                               /* [rows, D] of h_type, or packed (UITK_T_MX4) */
+    const void* gate;                      /* row m of the stream uses gate row m / gate_rows: 1 = per token, T = per sequence; or NULL */
+    const float* scale;                    /* [D] or NULL */
+    const float *post_w, *post_b;          /* [D]; NULL: no gain / no offset */
+    const float *pre_w, *pre_b;
+    int64_t rows, ldy, ldr, ldro, ldh, ldg, gate_rows;
+    int32_t D;                             /* 1 .. 16384 */
+    int32_t y_type, r_type, h_type, gate_type;
+    int32_t kind;                          /* uitk_norm, both norms */
+    int32_t post, pre;                     /* 0 / 1 */
+    float eps;
+} uitk_block_norm_args;
+int uitk_block_norm(const uitk_block_norm_args* a, void* stream);
+
 /* Last error message of the calling thread ("" if none). */
 const char* uitk_last_error(void);
 const char* uitk_version(void);

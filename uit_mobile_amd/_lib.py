@@ -15,6 +15,8 @@ IN_F32, IN_I16 = 0, 1
 PREC_F16, PREC_BF16, PREC_FP8, PREC_F16X2, PREC_F16L6, PREC_FP8W, PREC_F16A, PREC_F16AX, PREC_F32 = 0, 1, 2, 3, 4, 5, 6, 7, 8
 AVG_MEAN, AVG_MAX = 0, 1
 AMAX_SLOTS = 64
+T_F32, T_F16, T_BF16, T_MX4 = 0, 1, 2, 3
+NORM_LAYER, NORM_RMS = 0, 1
 
 EXPORTS = ["uitk_create", "uitk_destroy", "uitk_pack_weights", "uitk_num_frames", "uitk_num_crops",
            "uitk_reserve", "uitk_forward", "uitk_frontend", "uitk_amax_ptr", "uitk_encode", "uitk_mel_db",
@@ -22,7 +24,8 @@ EXPORTS = ["uitk_create", "uitk_destroy", "uitk_pack_weights", "uitk_num_frames"
            "uitk_version", "uitk_calibrate_weights", "uitk_calib_stats_doubles", "uitk_get_calib_stats", "uitk_pack_weights_calibrated",
            "uitk_tune_frontend", "uitk_get_calib_check", "uitk_self_check", "uitk_deviation_stats",
            "uitk_general_create", "uitk_general_destroy", "uitk_general_num_frames", "uitk_general_num_crops", "uitk_general_reserve",
-           "uitk_general_frontend", "uitk_general_amax_ptr", "uitk_general_encode", "uitk_general_forward", "uitk_general_mel_db"]
+           "uitk_general_frontend", "uitk_general_amax_ptr", "uitk_general_encode", "uitk_general_forward", "uitk_general_mel_db",
+           "uitk_mx4_bytes", "uitk_mx4_quantize", "uitk_mx4_dequantize", "uitk_mx4_linear_workspace", "uitk_mx4_linear", "uitk_block_norm"]
 
 
 class Config(Structure):
@@ -45,6 +48,17 @@ class BlockWeights(Structure):
 class Weights(Structure):
     _fields_ = [(n, c_void_p) for n in _GLOBAL_FIELDS] + [("blocks", POINTER(BlockWeights)), ("cls_token", c_void_p),
                                                           ("token_pos", c_void_p)]
+
+
+class Mx4LinearArgs(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "residual", "out", "workspace")] + [(n, c_int64) for n in ("M", "N", "K", "ldx", "ldr", "ldo")]
+                + [(n, c_int32) for n in ("x_type", "out_type", "act", "reserved")])
+
+
+class BlockNormArgs(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("y", "residual", "residual_out", "h", "gate", "scale", "post_w", "post_b", "pre_w", "pre_b")]
+                + [(n, c_int64) for n in ("rows", "ldy", "ldr", "ldro", "ldh", "ldg", "gate_rows")]
+                + [(n, c_int32) for n in ("D", "y_type", "r_type", "h_type", "gate_type", "kind", "post", "pre")] + [("eps", c_float)])
 
 
 _lib = None
@@ -99,6 +113,14 @@ def load():
     L.uitk_general_encode.argtypes = [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
     L.uitk_general_forward.argtypes = [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
     L.uitk_general_mel_db.argtypes = [c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p]
+    L.uitk_mx4_bytes.argtypes = [c_int64, c_int64]
+    L.uitk_mx4_bytes.restype = c_int64
+    L.uitk_mx4_quantize.argtypes = [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p]
+    L.uitk_mx4_dequantize.argtypes = [c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p]
+    L.uitk_mx4_linear_workspace.argtypes = [c_int64, c_int64, c_int64, c_int]
+    L.uitk_mx4_linear_workspace.restype = c_int64
+    L.uitk_mx4_linear.argtypes = [POINTER(Mx4LinearArgs), c_void_p]
+    L.uitk_block_norm.argtypes = [POINTER(BlockNormArgs), c_void_p]
     for name in EXPORTS:                      # every entry point include/uitk.h declares must be exported
         getattr(L, name)
     _lib = L

@@ -14,7 +14,10 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libuitk.so"
-SOURCES = ["api.cpp", "pack.cpp", "frontend.hip", "encoder.hip", "epilogue.hip", "calibrate.hip", "general.hip"]
+SOURCES = ["api.cpp", "pack.cpp", "frontend.hip", "encoder.hip", "epilogue.hip", "calibrate.hip", "general.hip", "mx4.hip", "block_norm.hip"]
+# sources whose fp32 math stays scalar: no packed v_pk_{add,mul,fma}_f32 (hipcc's host pass does not know the feature and says so)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"mx4.hip": NO_PACKED_F32, "block_norm.hip": NO_PACKED_F32}
 def _headers():
     """every header a translation unit can include: csrc/*.h (globbed: a new header cannot be forgotten -- naive_forward.h once was, and
     its structs travel by value between api.cpp and calibrate.hip) + the public C ABI"""
@@ -52,13 +55,13 @@ def build(force=False, verbose=False, extra_flags=()):
     compile_flags = [f for f in FLAGS if f != "-shared"]
     hdr_t = max((CSRC / h).stat().st_mtime for h in HEADERS)
     tag = obj_dir / "flags.txt"                               # other flags (lab builds) invalidate every object
-    flag_key = " ".join([*compile_flags, *extra_flags])
+    flag_key = " ".join([*compile_flags, *extra_flags, repr(SOURCE_FLAGS)])
     stale_all = force or not tag.exists() or tag.read_text() != flag_key
     jobs = []
     for s in SOURCES:
         obj = obj_dir / (s + ".o")
         if stale_all or not obj.exists() or obj.stat().st_mtime < max((CSRC / s).stat().st_mtime, hdr_t):
-            jobs.append([hipcc(), *compile_flags, *extra_flags, "-c", "-o", str(obj), str(CSRC / s)])
+            jobs.append([hipcc(), *compile_flags, *SOURCE_FLAGS.get(s, []), *extra_flags, "-c", "-o", str(obj), str(CSRC / s)])
 
     def run(cmd):
         if verbose:

@@ -1,0 +1,200 @@
+"""Microscaled 4-bit matrices (OCP MXFP4) and the linear layer on them: HIP kernels of libuitk.so (csrc/mx4.hip).
+
+`quantize(x)`      -> `Mx4Tensor`: 32 consecutive elements of the last dimension share a power-of-two scale (8 bits), an element is one of
+                     +-{0, .5, 1, 1.5, 2, 3, 4, 6} times it: 4.25 bits an element.  A block holding an infinity or a NaN is NaN as a whole.
+`Mx4Tensor.dequantize()`  the values the codes stand for
+`linear(x, w)`     = residual + act(Q(x) @ W.T + bias) on the 4-bit matrix pipe; the sums are fp32, the output is rounded once.  `x` a tensor
+                     (rounded to 4 bits on the way in) or an `Mx4Tensor`; `w` an `Mx4Tensor`, made once from the weights with `quantize`
+
+What `UITBase(precision='mx4')` runs its dense layers on (uit_mobile_amd/models/uit.py).  CUDA tensors only, on the tensors' device and its
+current stream; enqueue-only, safe inside a HIP graph capture.  No gradients: like the rest of this package these are inference operators,
+and a call that autograd would have to record is refused.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
+_ACTS = {None: 0, "relu": 1, "gelu": 2}
+
+
+def _ptr(t):
+    return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _stream(device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def check_tensor(t, name, dtypes=tuple(_TYPES)):
+    """A CUDA tensor of one of `dtypes` that needs no gradient (shared with norms.py)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor: uit_mobile_amd has no CPU path")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient: this is an inference operator (call it under torch.no_grad())")
+
+
+def as_rows(t):
+    """[..., K] -> (tensor [rows, K] whose last dimension is contiguous, its row stride): a view where the strides allow, else a copy."""
+    K = t.shape[-1]
+    rows = t.numel() // K if K else 0
+    v = t.view(rows, K) if t.is_contiguous() else t.reshape(rows, K)
+    if K > 1 and v.stride(1) != 1 or rows > 1 and v.stride(0) < K:
+        v = v.contiguous()
+    return v, (v.stride(0) if rows > 1 else K)
+
+
+def overlaps(a, b):
+    """Do two CUDA tensors share memory?  (By the spans their strides reach over: rows of one buffer that interleave count as sharing.)"""
+    def span(t):
+        lo = t.data_ptr()
+        return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if a.device != b.device or not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def check_vector(t, name, n, device):
+    """A per-channel parameter: [n] on `device`, handed on in float32."""
+    if t is None:
+        return None
+    check_tensor(t, name)
+    if t.shape != (n,):
+        raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return t.detach().to(torch.float32).contiguous()
+
+
+class Mx4Tensor:
+    """A packed 4-bit matrix: `shape` is the logical shape (blocks run along the last dimension), `data` the packed bytes -- an opaque
+    order made for the matrix pipe (csrc/mx4_dev.h)."""
+
+    def __init__(self, data, shape):
+        self.data = data
+        self.shape = torch.Size(shape)
+
+    @classmethod
+    def empty(cls, shape, device):
+        rows, K = math.prod(shape[:-1]), shape[-1]
+        n = _lib.load().uitk_mx4_bytes(rows, K)
+        if n < 0:
+            raise ValueError(f"a packed 4-bit matrix of {rows} rows x {K} is out of range (rows <= 2^31, 1 <= K <= 2^20)")
+        return cls(torch.empty(n, dtype=torch.uint8, device=device), shape)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def rows(self):
+        return math.prod(self.shape[:-1])
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def __repr__(self):
+        return f"Mx4Tensor({tuple(self.shape)}, device='{self.device}')"
+
+    def dequantize(self, dtype=torch.float32):
+        """The values, in `dtype` (exact in float32 and bfloat16; float16 rounds where a block's scale is out of its range)."""
+        if dtype not in _TYPES:
+            raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            with torch.cuda.device(self.device):
+                _lib.check(_lib.load().uitk_mx4_dequantize(_ptr(self.data), self.rows, self.shape[-1], _ptr(out), _TYPES[dtype], self.shape[-1],
+                                                           _stream(self.device)), "uitk_mx4_dequantize")
+        return out
+
+
+def quantize(x):
+    """x [..., K] (float32 / float16 / bfloat16) -> Mx4Tensor of the same shape."""
+    check_tensor(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., K] with K >= 1, got {tuple(x.shape)}")
+    q = Mx4Tensor.empty(x.shape, x.device)
+    if x.numel():
+        v, ld = as_rows(x.detach())
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.load().uitk_mx4_quantize(_ptr(v), _TYPES[v.dtype], v.shape[0], v.shape[1], ld, _ptr(q.data), _stream(x.device)),
+                       "uitk_mx4_quantize")
+    return q
+
+
+def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
+    """residual + act(Q(x) @ w.T + bias): x [..., K] tensor or Mx4Tensor, w Mx4Tensor [N, K], bias [N], act None / 'relu' / 'gelu' (exact),
+    residual [..., N] of the output's type -> [..., N].
+
+    out_dtype: float32 / float16 / bfloat16 (default: x's type, or the residual's; float32 for a packed x), or 'mx4': the output is an
+    Mx4Tensor, the next layer's x (no residual then).  out: write there instead (a contiguous tensor of the output's shape and type;
+    `out=residual` accumulates in place)."""
+    packed = isinstance(x, Mx4Tensor)
+    if not packed:
+        check_tensor(x, "x")
+    if not isinstance(w, Mx4Tensor):
+        raise TypeError("w must be an Mx4Tensor: quantize(weight) once")
+    if len(w.shape) != 2:
+        raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
+    if len(x.shape) < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} does not match w {tuple(w.shape)}")
+    if w.device != x.device:
+        raise ValueError(f"w is on {w.device}, x on {x.device}")
+    if act not in _ACTS:
+        raise ValueError(f"act must be None, 'relu' or 'gelu', got {act!r}")
+    device, (N, K) = x.device, w.shape
+    shape = tuple(x.shape[:-1]) + (N,)
+    M = math.prod(x.shape[:-1])
+    if residual is not None:
+        check_tensor(residual, "residual")
+    if out is not None and not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a tensor")
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.float32 if packed else x.dtype
+    to_mx4 = out_dtype == "mx4"
+    if not to_mx4 and out_dtype not in _TYPES:
+        raise TypeError(f"out_dtype must be float32, float16, bfloat16 or 'mx4', got {out_dtype}")
+    if residual is not None:
+        if to_mx4:
+            raise ValueError("a residual needs an output of 16 or 32 bits")
+        if residual.shape != shape or residual.dtype != out_dtype or residual.device != device:
+            raise ValueError(f"residual must be {shape} {out_dtype} on {device}, got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+    if out is not None:
+        if to_mx4:
+            raise ValueError("out is not supported for a 4-bit output")
+        check_tensor(out, "out")
+        if tuple(out.shape) != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {shape} {out_dtype} on {device}")
+        for name, t in (("x", x.data if packed else x), ("w", w.data), ("bias", bias)):
+            if t is not None and overlaps(out, t):
+                raise ValueError(f"out shares memory with {name}")
+        if residual is not None and overlaps(out, residual) and not (out.data_ptr() == residual.data_ptr() and residual.is_contiguous()):
+            raise ValueError("out shares memory with the residual without being the residual")
+    b = check_vector(bias, "bias", N, device)
+    if to_mx4:
+        result = Mx4Tensor.empty(shape, device)
+        dst, ldo = result.data, 0
+    else:
+        result = dst = torch.empty(shape, dtype=out_dtype, device=device) if out is None else out
+        ldo = N
+    if M == 0:
+        return result
+    L = _lib.load()
+    x_type = _lib.T_MX4 if packed else _TYPES[x.dtype]
+    src, ldx = (x.data, 0) if packed else as_rows(x.detach())
+    res, ldr = (None, 0) if residual is None else as_rows(residual.detach())
+    need = L.uitk_mx4_linear_workspace(M, N, K, x_type)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    a = _lib.Mx4LinearArgs(x=_ptr(src), w=_ptr(w.data), bias=_ptr(b), residual=_ptr(res), out=_ptr(dst), workspace=_ptr(ws), M=M, N=N, K=K,
+                           ldx=ldx, ldr=ldr, ldo=ldo, x_type=x_type, out_type=_lib.T_MX4 if to_mx4 else _TYPES[out_dtype], act=_ACTS[act])
+    with torch.cuda.device(device):
+        _lib.check(L.uitk_mx4_linear(ctypes.byref(a), _stream(device)), "uitk_mx4_linear")
+    return result
