@@ -218,6 +218,51 @@ def test_linear_epilogue(M, N, K, act, out_dtype):
     check_linear(acc, x, w, None, act, res)
 
 
+# what the tile kernels take: more than 64 tiles of 128 x 128; at least 512 of 256 x 128 and K >= 2048 (ragged edges in every direction)
+TILES = [(1100, 1030, 130), (1024, 1280, 64), (3000, 520, 400), (16385, 513, 2049), (128 * 128, 1024, 2048)]
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", DTYPES)
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_linear_many_rows(M, N, K, packed, out_dtype):
+    """Against the 64-bit product of the operands' own values (that quantize is right is another test's business)."""
+    x, w = _rand((M, K), torch.bfloat16, seed=M + N).cuda(), mx4.quantize((_rand((N, K), torch.float32, seed=K, spread=0.3) * K ** -0.5).cuda())
+    bias, res = _rand((N,), torch.float32, seed=3).cuda(), _rand((M, N), out_dtype, seed=4).cuda()
+    xq = mx4.quantize(x)
+    a, b = xq.dequantize().double(), w.dequantize().double()
+    S = a.abs() @ b.abs().T + bias.double().abs()
+    tol = (2 * math.ceil(K / 64) + 16) * 2.0 ** -23 * S
+    lin = a @ b.T + bias.double()
+    fi = torch.finfo(out_dtype)
+    for act, residual in ((None, None), ("relu", res), ("gelu", None)):
+        got = mx4.linear(xq if packed else x, w, bias=bias, act=act, residual=residual, out_dtype=out_dtype).double()
+        y, t = _act64(lin, act), tol
+        if act == "gelu":
+            t = 1.13 * tol + 2.0 ** -21 * y.abs().clamp(min=1.0)
+        if residual is not None:
+            y = y + residual.double()
+            t = tol + 2.0 ** -23 * y.abs()
+        assert ((got - y).abs() <= t + y.abs() * fi.eps / 2 + fi.smallest_normal * fi.eps).all(), act
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1100, 1030, 130), (16385, 260, 2049), (700, 2000, 256)])
+def test_linear_many_rows_to_four_bits_and_into_a_view(M, N, K):
+    x, w = mx4.quantize(_rand((M, K), torch.float16, seed=M).cuda()), mx4.quantize((_rand((N, K), torch.float32, seed=K) * K ** -0.5).cuda())
+    f = mx4.linear(x, w, act="relu", out_dtype=torch.float32)
+    q = mx4.linear(x, w, act="relu", out_dtype="mx4")
+    assert torch.equal(q.dequantize(), mx4.quantize(f).dequantize())
+    w2 = mx4.quantize((_rand((40, N), torch.float32, seed=1) * N ** -0.5).cuda())
+    assert torch.equal(mx4.linear(q, w2), mx4.linear(mx4.quantize(f), w2))
+    L = _lib.load()
+    buf = torch.full((M + 3, N + 8), 5.0, device="cuda")
+    a = _lib.Mx4LinearArgs(x=x.data.data_ptr(), w=w.data.data_ptr(), out=buf.data_ptr(), M=M, N=N, K=K, ldo=N + 8, x_type=3, out_type=0, act=1)
+    _lib.check(L.uitk_mx4_linear(ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), "linear")
+    assert (buf[M:] == 5.0).all() and (buf[:, N:] == 5.0).all() and torch.equal(buf[:M, :N], f)
+
+
 @gpu
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_linear_on_packed_activations_is_the_same_call(M, N, K):

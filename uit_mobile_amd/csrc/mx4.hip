@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "../../include/uitk.h"
 #include "mx4_dev.h"
@@ -85,12 +86,21 @@ struct Mx4LinearArgs {
     int vec4;                                                               // every four-element group of bias / residual / out is aligned
 };
 
+__device__ __forceinline__ mx_f4 mx4_bias4(const Mx4LinearArgs& a, int64_t n) {
+    mx_f4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (n + i < a.N) b[i] = a.bias[n + i];
+    }
+    return b;
+}
+
 // four consecutive outputs (row m, columns n ..): bias, activation, residual, one rounding, store
-__device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, int64_t n, float (&v)[4]) {
+__device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, int64_t n, const mx_f4& bias, float (&v)[4]) {
     const bool in_m = m < a.M;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (a.bias && n + i < a.N) v[i] += a.bias[n + i];
+        v[i] += bias[i];
         if (a.act == 1) v[i] = v[i] > 0.f ? v[i] : (v[i] != v[i] ? v[i] : 0.f);              // a NaN stays one
         else if (a.act == 2) v[i] = mx4_gelu(v[i]);
     }
@@ -214,7 +224,269 @@ __global__ void __launch_bounds__(256) mx4_linear_kernel(Mx4LinearArgs a) {
 #pragma unroll
         for (int w = 1; w < NW; ++w) s += *(const mx_f4*)&red[w][t][n4];
         float v[4] = {s[0], s[1], s[2], s[3]};
-        mx4_store4(a, m0 + t, ng * 64 + n4, v);
+        mx4_store4(a, m0 + t, ng * 64 + n4, mx4_bias4(a, ng * 64 + n4), v);
+    }
+}
+
+// ---- many rows: both operands packed, a workgroup computes BN outputs x BM tokens from LDS.
+// A stage holds 128 elements of K: BN / 64 + BM / 64 records, brought in by LDS-DMA in the order they have in memory (a record IS its
+// LDS image: every fragment read is 1 KB of consecutive bytes, no bank conflicts, no address arithmetic).  Three slots: while the waves
+// multiply stage s, stages s + 1 and s + 2 are on their way; the slot of s is free once its second half is in registers.
+// One barrier per stage, placed between the two halves: the fragments of the half in front of it are in registers already, so the
+// matrix pipe has work while the waves meet.
+__device__ __forceinline__ void mx4_dma16(unsigned lds, unsigned off, const char* src) {       // 64 lanes x 16 B -> 1 KB at lds
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void mx4_dma4(unsigned lds, unsigned off, const char* src) {        // 64 lanes x 4 B -> 256 B at lds
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(src) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void mx4_wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <int BN, int BM, int WN, int WM>                                   // WN x WM waves
+struct Mx4Tile {
+    static constexpr int NW = WN * WM, THREADS = 64 * NW;
+    static constexpr int RN = BN / 64, RM = BM / 64, REC = RN + RM;         // records of a stage
+    static constexpr int TN = BN / WN / 32, TM = BM / WM / 32;              // 32 x 32 tiles of a wave
+    static constexpr int STAGE = REC * (MX4_CODES + MX4_SCALES);
+    static constexpr int SLOTS = 3;
+    static constexpr int CP = REC * 4 / NW, SP = (REC + NW - 1) / NW;       // pieces of codes (1 KB) / of scales (256 B) a wave brings in per stage
+    static constexpr int LOADS = CP + SP;
+    static constexpr int LDE = TN * 32 + 4;                                 // floats per token row of the epilogue's buffer
+    static constexpr int EPI = NW * 32 * LDE * 4;
+    static constexpr int LDS = SLOTS * STAGE > EPI ? SLOTS * STAGE : EPI;
+    static_assert(REC * 4 % NW == 0, "every wave brings in the same number of pieces");
+};
+
+// ---- a wave's 32 tokens x 32 TN outputs, from its part of LDS to memory.  n0, m0: the first column / row; bias added, activation, residual
+// added, one rounding.  Whole tiles of aligned rows go four columns a lane; what sticks out or is not aligned goes one column a lane.
+template <int OUT> struct Mx4Out;
+template <> struct Mx4Out<MT_F32> {
+    typedef float T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const float* r) { const mx_f4 t = *(const mx_f4*)r; v[0] += t[0]; v[1] += t[1]; v[2] += t[2]; v[3] += t[3]; }
+    static __device__ __forceinline__ void put4(float* o, const float (&v)[4]) { *(mx_f4*)o = mx_f4{v[0], v[1], v[2], v[3]}; }
+};
+template <> struct Mx4Out<MT_F16> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const _Float16* r) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));            // (a bit cast of ONE element of a vector reads element 0, whichever was named)
+        const h4 t = *(const h4*)r;
+        v[0] += (float)t[0]; v[1] += (float)t[1]; v[2] += (float)t[2]; v[3] += (float)t[3];
+    }
+    static __device__ __forceinline__ void put4(_Float16* o, const float (&v)[4]) {
+        const mx_h2 a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
+        *(mx_u2*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    }
+};
+template <> struct Mx4Out<MT_BF16> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const __bf16* r) {
+        const mx_u2 t = *(const mx_u2*)r;
+        v[0] += __uint_as_float(t[0] << 16); v[1] += __uint_as_float(t[0] & 0xffff0000u); v[2] += __uint_as_float(t[1] << 16); v[3] += __uint_as_float(t[1] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void put4(__bf16* o, const float (&v)[4]) {
+        const mx_b2 a = {(__bf16)v[0], (__bf16)v[1]}, b = {(__bf16)v[2], (__bf16)v[3]};
+        *(mx_u2*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    }
+};
+
+template <int ACT> __device__ __forceinline__ float mx4_act(float v) {
+    if constexpr (ACT == 1) return v < 0.f ? 0.f : v;                       // (a NaN stays one)
+    else if constexpr (ACT == 2) return mx4_gelu(v);
+    else return v;
+}
+
+template <int OUT, int COLS, int LDE, int ACT>
+__device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const float* ep, int64_t m0, int64_t n0) {
+    const int lane = threadIdx.x & 63;
+    constexpr int LPR = COLS / 4, RPI = 64 / LPR;                           // lanes that hold a row, rows an instruction stores
+    if constexpr (OUT == MT_MX4) {
+        const int64_t n = n0 + (lane % LPR) * 4;
+        if (n0 >= a.out_S * MX4_K) return;
+        const mx_f4 bias = mx4_bias4(a, n);
+        const bool inside = n0 + COLS <= a.N;
+#pragma unroll 4
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int t = it * RPI + lane / LPR;
+            const mx_f4 w = *(const mx_f4*)&ep[t * LDE + (lane % LPR) * 4];
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = mx4_act<ACT>(w[i] + bias[i]); if (!inside && n + i >= a.N) v[i] = 0.f; }
+            unsigned sc;
+            const unsigned two = mx4_pack_quads(v, &sc);                    // (every lane is here: the 8 lanes of a block exchange their maxima)
+            if (m0 + t < a.M) {
+                const Mx4Place p = mx4_place(m0 + t, n >> 5, a.out_S);
+                *(unsigned short*)((char*)a.out + p.code + ((n & 31) >> 1)) = (unsigned short)two;
+                if ((n & 31) == 0) a.out_scales[p.scale] = (char)sc;
+            }
+        }
+    } else {
+        typedef typename Mx4Out<OUT>::T T;
+        if (m0 >= a.M || n0 >= a.N) return;
+        if (a.vec4 && n0 + COLS <= a.N && m0 + 32 <= a.M) {
+            const int64_t n = n0 + (lane % LPR) * 4;
+            const mx_f4 bias = mx4_bias4(a, n);
+            T* o = (T*)a.out + (m0 + lane / LPR) * a.ldo + n;
+            const T* r = a.residual ? (const T*)a.residual + (m0 + lane / LPR) * a.ldr + n : nullptr;
+#pragma unroll 4
+            for (int it = 0; it < 32 / RPI; ++it) {
+                const mx_f4 w = *(const mx_f4*)&ep[(it * RPI + lane / LPR) * LDE + (lane % LPR) * 4];
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = mx4_act<ACT>(w[i] + bias[i]);
+                if (r) Mx4Out<OUT>::add4(v, r + it * RPI * a.ldr);
+                Mx4Out<OUT>::put4(o + it * RPI * a.ldo, v);
+            }
+        } else {
+            const int rows = (int)min((int64_t)32, a.M - m0);
+#pragma unroll
+            for (int c = 0; c < COLS / 64; ++c) {
+                const int64_t n = n0 + c * 64 + lane;
+                if (n >= a.N) continue;
+                const float bias = a.bias ? a.bias[n] : 0.f;
+                T* o = (T*)a.out + m0 * a.ldo + n;
+                const T* r = a.residual ? (const T*)a.residual + m0 * a.ldr + n : nullptr;
+                for (int t = 0; t < rows; ++t) {
+                    float v = mx4_act<ACT>(ep[t * LDE + c * 64 + lane] + bias);
+                    if (r) v += (float)r[t * a.ldr];
+                    o[t * a.ldo] = (T)v;
+                }
+            }
+        }
+    }
+}
+
+template <int BN, int BM, int WN, int WM, int OUT>
+__global__ void __launch_bounds__(64 * WN * WM, BN * BM <= 256 * 128 ? 2 : 1) mx4_tile_kernel(Mx4LinearArgs a, int ntiles, int mtiles) {
+    typedef Mx4Tile<BN, BM, WN, WM> T;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // tiles in the order of their XCD (workgroup b runs on XCD b % 8), eight rows of tiles by columns: what an XCD works on at a time
+    // shares its operands in that XCD's L2
+    const int total = ntiles * mtiles;
+    int id = blockIdx.x;
+    { const int per = total / 8, rest = total % 8, x = id % 8; id = x * per + min(x, rest) + id / 8; }
+    constexpr int GRP = 8;
+    const int band = id / (GRP * ntiles), in_band = id - band * GRP * ntiles, bh = min(GRP, mtiles - band * GRP);
+    const int mt = band * GRP + in_band % bh, nt = in_band / bh;
+    const int S = (int)a.S;
+    const int64_t nrec = (a.N + MX4_ROWS - 1) / MX4_ROWS, mrec = (a.M + MX4_ROWS - 1) / MX4_ROWS;
+    // the pieces this wave brings in, at the same place of every stage (a tile's missing rows read the last record)
+    auto record = [&](int rec, bool scales) {
+        const bool is_w = rec < T::RN;
+        const int64_t g = is_w ? min((int64_t)nt * T::RN + rec, nrec - 1) : min((int64_t)mt * T::RM + rec - T::RN, mrec - 1);
+        return scales ? (is_w ? a.w_scales : a.x_scales) + g * S * MX4_SCALES : (is_w ? a.w : (const char*)a.x) + g * S * MX4_CODES;
+    };
+    const char* src_codes[T::CP];
+    const char* src_scales[T::SP];
+#pragma unroll
+    for (int i = 0; i < T::CP; ++i) src_codes[i] = record((wave * T::CP + i) / 4, false) + (wave * T::CP + i) % 4 * 1024;
+#pragma unroll
+    for (int i = 0; i < T::SP; ++i) src_scales[i] = record(min(wave * T::SP + i, T::REC - 1), true);
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const unsigned off16 = lane * 16, off4 = lane * 4;
+    auto bring = [&](int s) {
+        const unsigned slot = lds0 + (s % T::SLOTS) * T::STAGE;
+#pragma unroll
+        for (int i = 0; i < T::CP; ++i) mx4_dma16(slot + (wave * T::CP + i) * 1024, off16, src_codes[i] + (int64_t)s * MX4_CODES);
+#pragma unroll
+        for (int i = 0; i < T::SP; ++i)
+            mx4_dma4(slot + T::REC * MX4_CODES + min(wave * T::SP + i, T::REC - 1) * MX4_SCALES, off4, src_scales[i] + (int64_t)s * MX4_SCALES);
+    };
+    const int wn = wave / WM, wm = wave % WM;                               // the wave's place in the tile
+    // row tile j of the wave: rows 32 (wn TN + j) of the tile = record (..) / 2, half (..) % 2 of it.  TN and TM are even or the wave's
+    // first row tile is at an even place, so the byte of the scale dword is known at compile time
+    static_assert(T::TN % 2 == 0 && T::TM % 2 == 0, "a wave owns whole records");
+    mx_i4 fa[2][T::TN], fb[2][T::TM];
+    int sa[T::TN / 2], sb[T::TM / 2];
+    auto fetch = [&](int s, int kh, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM]) {
+        const char* slot = lds + (s % T::SLOTS) * T::STAGE;
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) A[j] = *(const mx_i4*)(slot + (wn * T::TN / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < T::TM; ++j) B[j] = *(const mx_i4*)(slot + (T::RN + wm * T::TM / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
+    };
+    auto fetch_scales = [&](int s, int (&A)[T::TN / 2], int (&B)[T::TM / 2]) {
+        const char* slot = lds + (s % T::SLOTS) * T::STAGE + T::REC * MX4_CODES;
+#pragma unroll
+        for (int j = 0; j < T::TN / 2; ++j) A[j] = *(const int*)(slot + (wn * T::TN / 2 + j) * MX4_SCALES + lane * 4);
+#pragma unroll
+        for (int j = 0; j < T::TM / 2; ++j) B[j] = *(const int*)(slot + (T::RN + wm * T::TM / 2 + j) * MX4_SCALES + lane * 4);
+    };
+    mx_f16 acc[T::TN][T::TM];
+#pragma unroll
+    for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TM; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    auto multiply = [&](auto KH, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM], int (&SA)[T::TN / 2], int (&SB)[T::TM / 2]) {
+        constexpr int kh = decltype(KH)::value;
+#pragma unroll
+        for (int i = 0; i < T::TN; i += 2)
+#pragma unroll
+            for (int j = 0; j < T::TM; j += 2) {
+                acc[i][j] = mx4_mfma<kh, kh>(A[i], B[j], acc[i][j], SA[i / 2], SB[j / 2]);
+                acc[i + 1][j] = mx4_mfma<2 + kh, kh>(A[i + 1], B[j], acc[i + 1][j], SA[i / 2], SB[j / 2]);
+                acc[i][j + 1] = mx4_mfma<kh, 2 + kh>(A[i], B[j + 1], acc[i][j + 1], SA[i / 2], SB[j / 2]);
+                acc[i + 1][j + 1] = mx4_mfma<2 + kh, 2 + kh>(A[i + 1], B[j + 1], acc[i + 1][j + 1], SA[i / 2], SB[j / 2]);
+            }
+    };
+    std::integral_constant<int, 0> K0;
+    std::integral_constant<int, 1> K1;
+    // ---- the pipeline
+    for (int s = 0; s < 3 && s < S; ++s) bring(s);
+    if (S >= 3) mx4_wait_dma<2 * T::LOADS>(); else if (S == 2) mx4_wait_dma<T::LOADS>(); else mx4_wait_dma<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch(0, 0, fa[0], fb[0]);
+    fetch_scales(0, sa, sb);
+    for (int s = 0; s + 1 < S; ++s) {
+        fetch(s, 1, fa[1], fb[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(K0, fa[0], fb[0], sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        // stage s + 1 has landed (this wave's part; the barrier says so for all), and this wave is done reading the slot of s
+        if (s + 2 < S) mx4_wait_dma<T::LOADS>(); else mx4_wait_dma<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 3 < S) bring(s + 3);
+        int oa[T::TN / 2], ob[T::TM / 2];                                   // the scales of the half that is still to be multiplied
+#pragma unroll
+        for (int i = 0; i < T::TN / 2; ++i) oa[i] = sa[i];
+#pragma unroll
+        for (int i = 0; i < T::TM / 2; ++i) ob[i] = sb[i];
+        fetch(s + 1, 0, fa[0], fb[0]);
+        fetch_scales(s + 1, sa, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(K1, fa[1], fb[1], oa, ob);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    fetch(S - 1, 1, fa[1], fb[1]);
+    multiply(K0, fa[0], fb[0], sa, sb);
+    multiply(K1, fa[1], fb[1], sa, sb);
+    __syncthreads();                                                        // every wave has left the ring
+    // ---- epilogue: 32 tokens at a time through the wave's own part of LDS, so that a lane holds four consecutive outputs of a token and
+    // a wave stores whole rows (straight from the accumulators a row would leave in pieces of 16 bytes)
+    float* ep = (float*)lds + wave * 32 * T::LDE;
+    const int c = lane & 31, g = lane >> 5;
+    const int64_t n0 = (int64_t)nt * BN + wn * T::TN * 32, mw = (int64_t)mt * BM + wm * T::TM * 32;
+#pragma unroll
+    for (int j = 0; j < T::TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *(mx_f4*)&ep[c * T::LDE + 32 * i + 8 * q + 4 * g] = mx_f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");              // (LDS serves a wave in order: what is left to do is to keep the compiler's)
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (a.act == 0) mx4_store_tile<OUT, T::TN * 32, T::LDE, 0>(a, ep, mw + 32 * j, n0);
+        else if (a.act == 1) mx4_store_tile<OUT, T::TN * 32, T::LDE, 1>(a, ep, mw + 32 * j, n0);
+        else mx4_store_tile<OUT, T::TN * 32, T::LDE, 2>(a, ep, mw + 32 * j, n0);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
 
@@ -246,6 +518,35 @@ static void mx4_launch_linear(dim3 grid, const Mx4LinearArgs& a, hipStream_t s) 
     else if (a.x_type == MT_F32) hipLaunchKernelGGL((mx4_linear_kernel<TT, float, false>), grid, dim3(256), 0, s, a);
     else if (a.x_type == MT_F16) hipLaunchKernelGGL((mx4_linear_kernel<TT, _Float16, false>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((mx4_linear_kernel<TT, __bf16, false>), grid, dim3(256), 0, s, a);
+}
+
+enum { MX4_SMALL = 0, MX4_TILE128 = 1, MX4_TILE256 = 2 };
+// Which kernel: few rows (or few tiles) are a matter of latency; the wide tile needs two workgroups on every CU, and a K long enough that its
+// longer epilogue does not matter (us, small / 128 x 128 / 256 x 128 tile: 1024 x 1024 x 1024: 7.0 / 7.7 / 17; 2048 x 2048 x 2048: 17.2 / 12.3 / 17;
+// 16128 x 2304 x 768: 112 / 32.8 / 38.1; 4096 x 4096 x 4096: 95 / 47.2 / 41.9; 8192 x 8192 x 8192: 658 / 304 / 281).
+static int mx4_choose(int64_t M, int64_t N, int64_t K) {
+    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), t256 = ((M + 127) / 128) * ((N + 255) / 256);
+    if (M <= 64 || t128 <= 64) return MX4_SMALL;
+    return t256 >= 512 && K >= 2048 ? MX4_TILE256 : MX4_TILE128;
+}
+
+template <int BN, int BM, int WN, int WM, int OUT>
+static hipError_t mx4_launch_tile_as(const Mx4LinearArgs& a, hipStream_t s) {
+    typedef Mx4Tile<BN, BM, WN, WM> T;
+    const int64_t cols = a.out_type == MT_MX4 ? a.out_S * MX4_K : a.N;
+    const int64_t nt = (cols + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
+    if (nt * mt > ((int64_t)1 << 32) / T::THREADS - 1) return hipErrorInvalidConfiguration;
+    if (T::LDS > 64 * 1024)                                                 // (of the current device: set at every call, not once per process)
+        if (hipError_t e = hipFuncSetAttribute((const void*)mx4_tile_kernel<BN, BM, WN, WM, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS); e != hipSuccess) return e;
+    hipLaunchKernelGGL((mx4_tile_kernel<BN, BM, WN, WM, OUT>), dim3((unsigned)(nt * mt)), dim3(T::THREADS), T::LDS, s, a, (int)nt, (int)mt);
+    return hipGetLastError();
+}
+template <int BN, int BM, int WN, int WM>
+static hipError_t mx4_launch_tile(const Mx4LinearArgs& a, hipStream_t s) {
+    if (a.out_type == MT_F32) return mx4_launch_tile_as<BN, BM, WN, WM, MT_F32>(a, s);
+    if (a.out_type == MT_F16) return mx4_launch_tile_as<BN, BM, WN, WM, MT_F16>(a, s);
+    if (a.out_type == MT_BF16) return mx4_launch_tile_as<BN, BM, WN, WM, MT_BF16>(a, s);
+    return mx4_launch_tile_as<BN, BM, WN, WM, MT_MX4>(a, s);
 }
 
 extern "C" {
@@ -296,10 +597,10 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     return UITK_OK;
 }
 
-// Activations that are not packed: quantised inside the product (few rows) -- no workspace so far
 int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type) {
     if (M < 0 || M > MX4_MAX_ROWS || N < 1 || N > MX4_MAX_K || K < 1 || K > MX4_MAX_K || x_type < UITK_T_F32 || x_type > UITK_T_MX4) return -1;
-    return 0;
+    // activations that are not packed: the tile kernels read them from a packed copy, the others quantise as they go
+    return x_type != UITK_T_MX4 && mx4_choose(M, N, K) != MX4_SMALL ? mx4_bytes(M, K) : 0;
 }
 
 int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
@@ -330,14 +631,31 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
         const int sz = type_size(u->out_type), grp = 4 * sz;
         a.vec4 = (uintptr_t)u->out % grp == 0 && u->ldo % 4 == 0 && (!u->residual || ((uintptr_t)u->residual % grp == 0 && u->ldr % 4 == 0));
     }
-    const int64_t ngroups = u->out_type == UITK_T_MX4 ? 2 * a.out_S : (u->N + MX4_ROWS - 1) / MX4_ROWS;
     hipStream_t s = (hipStream_t)stream;
-    const int tt = u->M <= 32 ? 1 : 2;
-    const int64_t mt = (u->M + 32 * tt - 1) / (32 * tt);
-    if (mt * ngroups > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
-    a.ngroups = (unsigned)ngroups;
-    const dim3 grid((unsigned)(mt * ngroups));
-    if (tt == 1) mx4_launch_linear<1>(grid, a, s); else mx4_launch_linear<2>(grid, a, s);
+#ifdef UITK_LAB
+    const int kind = u->reserved ? u->reserved - 1 : mx4_choose(u->M, u->N, u->K);
+#else
+    const int kind = mx4_choose(u->M, u->N, u->K);
+#endif
+    if (kind == MX4_SMALL) {
+        const int64_t ngroups = u->out_type == UITK_T_MX4 ? 2 * a.out_S : (u->N + MX4_ROWS - 1) / MX4_ROWS;
+        const int tt = u->M <= 32 ? 1 : 2;
+        const int64_t mt = (u->M + 32 * tt - 1) / (32 * tt);
+        if (mt * ngroups > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
+        a.ngroups = (unsigned)ngroups;
+        const dim3 grid((unsigned)(mt * ngroups));
+        if (tt == 1) mx4_launch_linear<1>(grid, a, s); else mx4_launch_linear<2>(grid, a, s);
+    } else {
+        if (u->x_type != UITK_T_MX4) {
+            if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
+            if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
+            a.x = u->workspace; a.x_type = MT_MX4; a.x_scales = (const char*)u->workspace + mx4_records(u->M, u->K) * MX4_CODES;
+        }
+        const hipError_t e = kind == MX4_TILE256 ? mx4_launch_tile<256, 128, 2, 2>(a, s) : mx4_launch_tile<128, 128, 2, 2>(a, s);
+        if (e == hipErrorInvalidConfiguration) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
+        MX4_HIP(e);
+        return UITK_OK;
+    }
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }

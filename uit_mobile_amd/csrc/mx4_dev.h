@@ -174,9 +174,19 @@ __device__ __forceinline__ mx_f16 mx4_mfma(mx_i4 a, mx_i4 b, mx_f16 c, int sa, i
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, SA, sa, SB, sb);
 }
 
-// x Phi(x), exact GELU
-__device__ __forceinline__ float mx4_gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-
-template <typename T> __device__ __forceinline__ float mx_to_f32(T v) { return (float)v; }
+// x Phi(x) (exact GELU): the upper tail 1 - Phi(|x|) = phi(x) (b1 t + .. + b5 t^5), t = 1 / (1 + p |x|), by formula 26.2.17 of Abramowitz and
+// Stegun's handbook: |error| <= 7.5e-8, about the half step of an fp32 Phi, in 12 instructions (erff: ~40; on 8192 x 8192 outputs the
+// epilogue is a visible share of the product)
+__device__ __forceinline__ float mx4_gelu(float x) {
+    const float ax = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.2316419f, ax, 1.0f));
+    float p = 1.330274429f;
+    p = fmaf(p, t, -1.821255978f);
+    p = fmaf(p, t, 1.781477937f);
+    p = fmaf(p, t, -0.356563782f);
+    p = fmaf(p, t, 0.319381530f);
+    // phi(x) = exp(-x^2 / 2) / sqrt(2 pi)
+    const float q = p * t * (0.3989422804f * __builtin_amdgcn_exp2f(-0.7213475204f * x * x));
+    return x * (x > 0.f ? 1.0f - q : q);
+}
 
 }  // namespace uitk
