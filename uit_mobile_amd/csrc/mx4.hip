@@ -44,29 +44,48 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
     *(unsigned*)(scales + rec * MX4_SCALES + lane * 4) = sc;
 }
 
-template <typename T>
+// One wave per record here too, but 16 lanes share a row: each turns four bytes of codes into eight elements, so that a wave stores 128
+// consecutive elements of four rows at a time (a whole block per lane would store 16-byte pieces 64 bytes apart).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales, int64_t rows, int64_t K, int64_t ld,
                                                              int64_t R, int64_t S, T* __restrict__ x) {
-    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, kb = l16 >> 2;      // the lane's block of its row: half kb / 2, group kb % 2
     const int64_t rec = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (rec >= R * S) return;
-    const int64_t rg = rec / S, s = rec - rg * S;
-    const unsigned sc = *(const unsigned*)(scales + rec * MX4_SCALES + lane * 4);
+    const int64_t rg = rec / S, s = rec - rg * S, k = s * MX4_K + l16 * 8;
+    const int n = (int)min((int64_t)8, K - k);
+    const char* c = codes + rec * MX4_CODES + (kb >> 1) * 1024 + (kb & 1) * 512 + (l16 & 3) * 4;
+    const unsigned char* sc = (const unsigned char*)scales + rec * MX4_SCALES + (kb & 1) * 128 + (kb >> 1);
+#pragma unroll 4
+    for (int it = 0; it < 16; ++it) {
+        const int r = it * 4 + (lane >> 4);                                 // 0 .. 63
+        const int64_t row = rg * MX4_ROWS + r;
+        const unsigned w = *(const unsigned*)(c + (r >> 5) * 2048 + (r & 31) * 16);
+        const unsigned b = sc[(r & 31) * 4 + 2 * (r >> 5)];
+        const float f = mx4_scale_float(b);
+        float v[8];
+        const mx_f2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 1);
+        const mx_f2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 3);
+        v[0] = v0[0]; v[1] = v0[1]; v[2] = v1[0]; v[3] = v1[1]; v[4] = v2[0]; v[5] = v2[1]; v[6] = v3[0]; v[7] = v3[1];
+        if (b == 255u) {
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        const int64_t row = rg * MX4_ROWS + 32 * (f >> 1) + r, k = s * MX4_K + 64 * (f & 1) + 32 * g;
-        if (row >= rows || k >= K) continue;
-        const mx_i4 c = *(const mx_i4*)(codes + rec * MX4_CODES + f * 1024 + lane * 16);
-        const unsigned byte = sc >> (8 * f) & 255u;
-        const int n = (int)min((int64_t)32, K - k);
-        T* out = x + row * ld + k;
-        // 2^(byte - 127) in two steps: half of it is never subnormal for byte >= 2, and for byte < 2 the products stay exact
-        for (int j = 0; j < n; ++j) {
-            const unsigned code = (unsigned)c[j >> 3] >> (4 * (j & 7)) & 15u;
-            const unsigned mag = code & 7u;
-            const float m = mag < 2u ? 0.5f * mag : __uint_as_float(((mag >> 1) + 126u) << 23 | (mag & 1u) << 22);
-            const float v = byte == 255u ? __uint_as_float(0x7fc00000u) : ldexpf(code & 8u ? -m : m, (int)byte - 127);
-            out[j] = (T)v;
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
+        }
+        if (row >= rows || n <= 0) continue;
+        T* o = x + row * ld + k;
+        if (VEC && n == 8) {
+            typedef T T8 __attribute__((ext_vector_type(16 / sizeof(T))));
+            constexpr int P = 16 / sizeof(T);                               // elements of a 16-byte store
+#pragma unroll
+            for (int h = 0; h < 8 / P; ++h) {
+                T8 t;
+#pragma unroll
+                for (int i = 0; i < P; ++i) t[i] = (T)v[h * P + i];
+                *(T8*)(o + h * P) = t;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i < n) o[i] = (T)v[i];
         }
     }
 }
@@ -590,9 +609,11 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     const char* scales = codes + R * S * MX4_CODES;
     const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (float*)x);
-    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_dequantize_kernel<_Float16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (_Float16*)x);
-    else hipLaunchKernelGGL(mx4_dequantize_kernel<__bf16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (__bf16*)x);
+    const bool vec = aligned16(x) && (ld * type_size(type)) % 16 == 0;
+    auto launch = [&](auto kernel, auto* out) { hipLaunchKernelGGL(kernel, grid, block, 0, s, codes, scales, rows, K, ld, R, S, out); };
+    if (type == UITK_T_F32) vec ? launch(mx4_dequantize_kernel<float, true>, (float*)x) : launch(mx4_dequantize_kernel<float, false>, (float*)x);
+    else if (type == UITK_T_F16) vec ? launch(mx4_dequantize_kernel<_Float16, true>, (_Float16*)x) : launch(mx4_dequantize_kernel<_Float16, false>, (_Float16*)x);
+    else vec ? launch(mx4_dequantize_kernel<__bf16, true>, (__bf16*)x) : launch(mx4_dequantize_kernel<__bf16, false>, (__bf16*)x);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }

@@ -140,14 +140,32 @@ template <> struct Mx4Src<__bf16> : Mx4Src16<__bf16> {
     }
 };
 
+// ---- reductions over neighbouring lanes without LDS: DPP within 16 lanes, row swaps beyond
+template <int CTRL> __device__ __forceinline__ unsigned mx_dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
+// every lane gets the result over its group of N lanes (4, 8, 16, 32 or 64)
+template <int N, typename F> __device__ __forceinline__ unsigned mx_lanes(unsigned v, F f) {
+    static_assert(N >= 4 && N <= 64 && (N & (N - 1)) == 0, "");
+    v = f(v, mx_dpp<DPP_XOR1>(v));
+    v = f(v, mx_dpp<DPP_XOR2>(v));
+    if constexpr (N >= 8) v = f(v, mx_dpp<DPP_HALF_MIRROR>(v));
+    if constexpr (N >= 16) v = f(v, mx_dpp<DPP_MIRROR>(v));
+    if constexpr (N >= 32) { const auto t = __builtin_amdgcn_permlane16_swap(v, v, false, false); v = f(t[0], t[1]); }
+    if constexpr (N >= 64) { const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false); v = f(t[0], t[1]); }
+    return v;
+}
+template <int N> __device__ __forceinline__ unsigned mx_lanes_max(unsigned v) { return mx_lanes<N>(v, [](unsigned a, unsigned b) { return max(a, b); }); }
+template <int N> __device__ __forceinline__ float mx_lanes_sum(float v) {
+    return __uint_as_float(mx_lanes<N>(__float_as_uint(v), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+
 // ---- packing inside an epilogue: 8 neighbouring lanes hold 4 consecutive elements of a block each.  -> the lane's two bytes of codes
 // and the block's scale byte (the same on the 8 lanes)
 __device__ __forceinline__ unsigned mx4_pack_quads(const float (&v)[4], unsigned* scale) {
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    m = mx_lanes_max<8>(m);
     const unsigned b = mx4_scale_byte(m >> 23);
     const float s = mx4_scale_float(b);
     unsigned w = 0;
@@ -155,6 +173,23 @@ __device__ __forceinline__ unsigned mx4_pack_quads(const float (&v)[4], unsigned
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
     *scale = b;
     return b == 255u ? 0u : w & 0xffffu;
+}
+
+// the same for 4 neighbouring lanes with 8 consecutive elements each -> the lane's four bytes of codes
+__device__ __forceinline__ unsigned mx4_pack_octets(const float* v, unsigned* scale) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    m = mx_lanes_max<4>(m);
+    const unsigned b = mx4_scale_byte(m >> 23);
+    const float s = mx4_scale_float(b);
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], s, 3);
+    *scale = b;
+    return b == 255u ? 0u : w;
 }
 
 // where block kb (32 elements) of row r lives in a packed matrix of S records per row group
