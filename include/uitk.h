@@ -77,6 +77,8 @@ typedef enum uitk_precision {
                            right for every checkpoint, e.g. those with strong attention sinks, whose fp16 activation floor no split
                            mode brings inside the budget (tools/err_attrib_sink.py).  get_option("parity_escalate_to") of a split-weight
                            handle (f16l6 / f16x2 / f16ax) that uitk_calibrate_weights measured over its budget names it */
+    UITK_PREC_MX4 = 9,  /* uitk_general_create only: the dense layers of the general engine's blocks on 4-bit operands (OCP MXFP4 weights AND activations,
+                           fp32 sums), everything else fp32 as in UITK_PREC_F32.  A measured throughput mode, far outside the parity gate */
     UITK_PREC_F16L6 = 4 /* round 3's parity mode (kept built and tested): fp16 operands as UITK_PREC_F16 plus the LOW-ORDER weight term on the cheap pipe:
                            W = f16(W) + 2^e(row) . e2m3(W - f16(W)), the second term as OCP fp6 on
                            v_mfma_scale_f32_16x16x128_f8f6f4 (one MFMA at the cost of one f16 k-step covers K = 128) against fp6
@@ -328,7 +330,8 @@ int uitk_kws_transform(float* y_pred, const float* y, int64_t B, int32_t C, int3
  * (models/uit.py:253-363: n_mels / n_fft / win_size / hop_size / center, patch_size (== stride), target_length, embed_dim, depth,
  * num_heads, mlp_ratio, both attention classes, ReLU / GELU, the three poolings) that the MFMA kernels above are NOT specialised to --
  * uitk_create refuses those (UITK_ERR_UNSUPPORTED).  Plain fp32 arithmetic on the device in the reference's order of operations (the
- * dense layers on the matrix pipe's exact-fp32 mode); cfg->precision must be UITK_PREC_F32; nothing to calibrate or tune.  The weights
+ * dense layers on the matrix pipe's exact-fp32 mode); cfg->precision UITK_PREC_F32, or UITK_PREC_MX4: the blocks' dense layers on 4-bit operands
+ * (a throughput mode); nothing to calibrate or tune.  The weights
  * use uitk_weights with the shapes the config implies: pe_w [embed, 1, P, P], time_pos [1, embed, 1, target_length / P],
  * freq_pos [1, embed, n_mels / P, 1], qkv_w [3 inner, embed] (inner = embed, or embed / 4 for BNeckAttention), proj_w [embed, inner],
  * fc1_w [mlp_hidden, embed], fc2_w [embed, mlp_hidden], head_w [outputdim, embed], mel_fb [n_fft / 2 + 1, n_mels], window [win_size].

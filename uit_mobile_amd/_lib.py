@@ -12,7 +12,7 @@ LIB_PATH = Path(os.environ["UITK_LIB_PATH"]) if os.environ.get("UITK_LIB_PATH") 
 UITK_OK = 0
 ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_NO_DEVICE, ERR_HIP, ERR_TOO_SHORT, ERR_WORKSPACE = -1, -2, -3, -4, -5, -6
 IN_F32, IN_I16 = 0, 1
-PREC_F16, PREC_BF16, PREC_FP8, PREC_F16X2, PREC_F16L6, PREC_FP8W, PREC_F16A, PREC_F16AX, PREC_F32 = 0, 1, 2, 3, 4, 5, 6, 7, 8
+PREC_F16, PREC_BF16, PREC_FP8, PREC_F16X2, PREC_F16L6, PREC_FP8W, PREC_F16A, PREC_F16AX, PREC_F32, PREC_MX4 = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
 AVG_MEAN, AVG_MAX = 0, 1
 AMAX_SLOTS = 64
 T_F32, T_F16, T_BF16, T_MX4 = 0, 1, 2, 3
@@ -125,6 +125,20 @@ def load():
         getattr(L, name)
     _lib = L
     return L
+
+
+_packed = {}
+
+
+def packed(name):
+    """The entry point `name` (struct pointer, stream) taking the struct as bytes: filling a ctypes Structure of thirty fields costs more
+    host time than the launch behind it."""
+    fn = _packed.get(name)
+    if fn is None:
+        fn = load()[name]                       # (a function object of its own: its argument types leave the attribute's alone)
+        fn.argtypes = [c_char_p, c_void_p]
+        _packed[name] = fn
+    return fn
 
 
 def last_error():

@@ -9,6 +9,10 @@
 // general-geometry sibling of precision 'f32' (calibrate.hip: launch_naive_forward): right first, an order of magnitude slower than
 // the MFMA encoder, two orders faster than the CPU path.  Never used for a configuration the MFMA kernels accept.
 //
+// Precision 'mx4' (UITK_PREC_MX4): the same network with the four dense layers of every block on 4-bit operands (mx4.hip: weights packed
+// at create, activations rounded on the way) and the seams between them -- residual add, LayerNorm, 4-bit rounding -- in one pass
+// (block_norm.hip).  Front-end, patch embed, attention, residual stream and head stay fp32.  A measured throughput mode, not a parity mode.
+//
 //   front-end   models/uit.py:298-308: torchaudio 0.13 MelSpectrogram + AmplitudeToDB(top_db=120), the batch-global floor applied by
 //               the consumer (gen_patch_kernel) once the whole call's amax is known -- as in the fast path
 //   patches     models/uit.py:460-462 (init_bn), :63-66 (Conv2d k = stride = patch), :381-392 (positional embeddings, cls token)
@@ -24,6 +28,7 @@
 #include <vector>
 
 #include "../../include/uitk.h"
+#include "mx4_dev.h"
 #include "naive_forward.h"
 #include "uitk_dev.h"
 
@@ -375,6 +380,7 @@ __global__ void __launch_bounds__(256) gen_head_kernel(const float* __restrict__
 // ------------------------------------------------------------------------------------------------------------------ host side + C ABI
 using namespace uitk;
 
+enum { GEN_QKV = 0, GEN_PROJ, GEN_FC1, GEN_FC2 };                         // the dense layers of a block
 struct GenBlockPtrs { const float *n1w, *n1b, *qkv_w, *qkv_b, *proj_w, *proj_b, *n2w, *n2b, *fc1_w, *fc1_b, *fc2_w, *fc2_b; };
 
 struct uitk_general {
@@ -391,7 +397,11 @@ struct uitk_general {
     float* frames = nullptr; size_t frames_cap = 0;
     float* work = nullptr; size_t work_cap = 0; int64_t work_rows = 0; int work_ntok = 0;
     float* rowprobs = nullptr; size_t rowprobs_cap = 0;
+    char* packed = nullptr;                  // precision 'mx4': the packed weights [depth][4 layers] ...
+    std::vector<size_t> packed_off;          // ... [4 b + layer] -> bytes into `packed`
+    float* work4 = nullptr; size_t work4_cap = 0;      // precision 'mx4': the packed operands of the chunk (gen_work4)
     int64_t fe_B = 0, fe_T = 0;
+    bool mx4() const { return cfg.precision == UITK_PREC_MX4; }
 };
 
 #define GEN_HIP(expr)                                                                                          \
@@ -416,7 +426,7 @@ static int gen_time_patches(const uitk_general* m, int64_t T) {
 
 static int gen_validate(const uitk_config* c, std::string* why) {
     auto bad = [&](const char* s) { *why = s; return UITK_ERR_UNSUPPORTED; };
-    if (c->precision != UITK_PREC_F32) return bad("the general engine computes in fp32: precision must be UITK_PREC_F32");
+    if (c->precision != UITK_PREC_F32 && c->precision != UITK_PREC_MX4) return bad("general engine: precision must be UITK_PREC_F32 (the engine computes in fp32) or UITK_PREC_MX4 (its dense layers on 4-bit operands)");
     if (c->n_fft < 16 || c->n_fft > 4096 || (c->n_fft & 1)) return bad("general engine: n_fft must be even, 16..4096");
     if ((c->n_fft & (c->n_fft - 1)) && c->n_fft > 2048) return bad("general engine: an n_fft that is no power of two must be <= 2048 (the DFT path keeps its twiddles in LDS)");
     if (c->win_size < 1 || c->win_size > c->n_fft) return bad("win_size must be 1..n_fft");
@@ -451,9 +461,19 @@ static int gen_check_shape(const uitk_general* m, int64_t B, int64_t T) {
     return UITK_OK;
 }
 
-// floats of work buffers per clip-crop with ntok tokens: X0 | R | Xn | QKV | O | Hd
-static size_t gen_row_floats(const GenGeom& g, int ntok) {
-    return (size_t)ntok * ((size_t)g.P * g.P + 2 * (size_t)g.D + 3 * (size_t)g.inner + g.inner + g.hidden);
+// floats of work buffers per clip-crop with ntok tokens: X0 | R | Xn | QKV | O | Hd (precision 'mx4': no Hd, it is 4-bit)
+static size_t gen_row_floats(const GenGeom& g, int ntok, bool mx4) {
+    return (size_t)ntok * ((size_t)g.P * g.P + 2 * (size_t)g.D + 3 * (size_t)g.inner + g.inner + (mx4 ? 0 : g.hidden));
+}
+// precision 'mx4', packed operands of M tokens: the norms' output | the MLP's hidden layer | the attention output (workspace of its product)
+struct GenWork4 { size_t h, hid, att, bytes; };
+static GenWork4 gen_work4(const GenGeom& g, int64_t M) {
+    GenWork4 w;
+    w.h = 0;
+    w.hid = w.h + (size_t)mx4_bytes(M, g.D);
+    w.att = w.hid + (size_t)mx4_bytes(M, g.hidden);
+    w.bytes = w.att + (size_t)mx4_bytes(M, g.inner);
+    return w;
 }
 constexpr size_t GEN_WORK_BYTES = (size_t)3 << 30;                        // rows are processed in chunks that fit this
 
@@ -558,6 +578,20 @@ int uitk_general_create(const uitk_config* cfg, const uitk_weights* w, uitk_gene
         const size_t* o = ob.data() + (size_t)b * 12;
         m->blocks[b] = GenBlockPtrs{p + o[0], p + o[1], p + o[2], p + o[3], p + o[4], p + o[5], p + o[6], p + o[7], p + o[8], p + o[9], p + o[10], p + o[11]};
     }
+    if (m->mx4()) {                          // pack the dense layers: on the device, from the fp32 copies just uploaded
+        const int64_t rows[4] = {3 * (int64_t)g.inner, D, g.hidden, D}, cols[4] = {D, g.inner, D, g.hidden};
+        size_t bytes = 0;
+        m->packed_off.resize((size_t)g.depth * 4);
+        for (int i = 0; i < g.depth * 4; ++i) { m->packed_off[i] = bytes; bytes += (size_t)mx4_bytes(rows[i % 4], cols[i % 4]); }
+        int rc = hipMalloc((void**)&m->packed, bytes) == hipSuccess ? UITK_OK : set_error(UITK_ERR_HIP, "general engine: no memory for the packed weights");
+        for (int i = 0; i < g.depth * 4 && rc == UITK_OK; ++i) {
+            const GenBlockPtrs& w4 = m->blocks[i / 4];
+            const float* src[4] = {w4.qkv_w, w4.proj_w, w4.fc1_w, w4.fc2_w};
+            rc = uitk_mx4_quantize(src[i % 4], UITK_T_F32, rows[i % 4], cols[i % 4], cols[i % 4], m->packed + m->packed_off[i], nullptr);
+        }
+        if (rc == UITK_OK && hipDeviceSynchronize() != hipSuccess) rc = set_error(UITK_ERR_HIP, "general engine: packing the weights failed");
+        if (rc != UITK_OK) { uitk_general_destroy(m); return rc; }
+    }
     float armed[AMAX_SLOTS];
     for (float& v : armed) v = -INFINITY;
     (void)hipMemcpy(m->amax, armed, sizeof armed, hipMemcpyHostToDevice);
@@ -572,6 +606,8 @@ int uitk_general_destroy(uitk_general* m) {
     if (m->frames) (void)hipFree(m->frames);
     if (m->work) (void)hipFree(m->work);
     if (m->rowprobs) (void)hipFree(m->rowprobs);
+    if (m->packed) (void)hipFree(m->packed);
+    if (m->work4) (void)hipFree(m->work4);
     delete m;
     return UITK_OK;
 }
@@ -586,12 +622,15 @@ static int gen_reserve(uitk_general* m, int64_t B, int64_t T, hipStream_t s) {
     const int ntok = m->g.GF * nt + m->g.cls;
     if (int rc = gen_grow(&m->frames, &m->frames_cap, (size_t)B * nF * m->g.M * 4, s)) return rc;
     const int64_t rows = B * nc;
-    const size_t per_row = gen_row_floats(m->g, ntok) * 4;
+    const size_t per_row = gen_row_floats(m->g, ntok, m->mx4()) * 4;
     int64_t chunk = (int64_t)std::max<size_t>(1, GEN_WORK_BYTES / per_row);
     chunk = std::min<int64_t>(chunk, rows);
     chunk = std::min<int64_t>(chunk, (int64_t)65535 * 64 / ntok);          // the dense kernel's grid: 64 token rows per workgroup in gridDim.y
     if (chunk < 1) return set_error(UITK_ERR_UNSUPPORTED, "general engine: one clip-crop exceeds the work buffer");
     if (int rc = gen_grow(&m->work, &m->work_cap, (size_t)chunk * per_row, s)) return rc;
+    // (work_rows below can exceed this call's chunk where an earlier shape grew the buffer; the packed operands follow it)
+    if (m->mx4())
+        if (int rc = gen_grow(&m->work4, &m->work4_cap, gen_work4(m->g, std::min<int64_t>((int64_t)(m->work_cap / per_row), rows) * ntok).bytes, s)) return rc;
     m->work_rows = (int64_t)(m->work_cap / per_row); m->work_ntok = ntok;
     if (int rc = gen_grow(&m->rowprobs, &m->rowprobs_cap, nc > 1 ? (size_t)rows * m->g.C * 4 : 0, s)) return rc;
     return UITK_OK;
@@ -620,6 +659,55 @@ int uitk_general_frontend(uitk_general* m, const void* pcm, int in_dtype, int64_
     if (int rc = gen_reserve(m, B, T, (hipStream_t)stream)) return rc;
     if (int rc = gen_run_frontend(m, pcm, in_dtype, B, T, (hipStream_t)stream)) return rc;
     m->fe_B = B; m->fe_T = T;
+    return UITK_OK;
+}
+
+static hipError_t gen_attention(const float* QKV, float* O, int n, const GenGeom& g, float scale, hipStream_t s) {
+    if (g.hd <= 8) gen_launch_attention<8>(QKV, O, n, g, g.ntok, scale, s);
+    else if (g.hd <= 16) gen_launch_attention<16>(QKV, O, n, g, g.ntok, scale, s);
+    else if (g.hd <= 32) gen_launch_attention<32>(QKV, O, n, g, g.ntok, scale, s);
+    else if (g.hd <= 64) gen_launch_attention<64>(QKV, O, n, g, g.ntok, scale, s);
+    else if (g.hd <= 128) gen_launch_attention<128>(QKV, O, n, g, g.ntok, scale, s);
+    else hipLaunchKernelGGL(gen_attention_wide_kernel, dim3(n * g.heads, (g.ntok + 63) / 64, (g.hd + 63) / 64), dim3(64), 0, s, QKV, O, g.ntok, g.heads, g.inner, g.hd, scale);
+    return hipGetLastError();
+}
+
+// precision 'mx4': the blocks of n clip-crops and the final norm.  R: the fp32 residual stream; Xn receives the blocks' outputs on their
+// way into it and, last, norm(R) for the head.  Every dense layer reads 4-bit activations: the norms and the MLP's first layer write
+// them, the attention's output is rounded by its product.
+static int gen_blocks_mx4(uitk_general* m, const GenGeom& g, int n, float* R, float* Xn, float* QKV, float* O, float scale, hipStream_t s) {
+    const int64_t M = (int64_t)n * g.ntok;
+    const GenWork4 w4 = gen_work4(g, M);
+    if (w4.bytes > m->work4_cap) return set_error(UITK_ERR_WORKSPACE, "general engine: no workspace for the packed operands of this shape");
+    char* h = (char*)m->work4 + w4.h;
+    char* hid = (char*)m->work4 + w4.hid;
+    char* att = (char*)m->work4 + w4.att;
+    // R += y (y null: as it is); out = LayerNorm(R)
+    auto seam = [&](const float* y, const float* w, const float* b, void* out, int type) {
+        uitk_block_norm_args a{};
+        a.y = y; a.residual = R; a.residual_out = y ? R : nullptr; a.h = out; a.pre = 1; a.pre_w = w; a.pre_b = b;
+        a.rows = M; a.D = g.D; a.ldy = a.ldr = a.ldro = a.ldh = g.D; a.gate_rows = 1;
+        a.y_type = a.r_type = UITK_T_F32; a.h_type = type; a.kind = UITK_NORM_LAYER; a.eps = 1e-6f;
+        return uitk_block_norm(&a, s);
+    };
+    auto linear = [&](const void* x, int x_type, int64_t K, int layer, int b, const float* bias, int act, void* out, int out_type, int64_t N) {
+        uitk_mx4_linear_args a{};
+        a.x = x; a.x_type = x_type; a.ldx = K; a.w = m->packed + m->packed_off[4 * (size_t)b + layer]; a.bias = bias; a.act = act; a.out = out; a.out_type = out_type;
+        a.ldo = N; a.M = M; a.N = N; a.K = K; a.workspace = att;
+        return uitk_mx4_linear(&a, s);
+    };
+    if (int rc = seam(nullptr, m->blocks[0].n1w, m->blocks[0].n1b, h, UITK_T_MX4)) return rc;
+    for (int b = 0; b < g.depth; ++b) {
+        const GenBlockPtrs& w = m->blocks[b];
+        if (int rc = linear(h, UITK_T_MX4, g.D, GEN_QKV, b, w.qkv_b, 0, QKV, UITK_T_F32, 3 * g.inner)) return rc;
+        GEN_HIP(gen_attention(QKV, O, n, g, scale, s));
+        if (int rc = linear(O, UITK_T_F32, g.inner, GEN_PROJ, b, w.proj_b, 0, Xn, UITK_T_F32, g.D)) return rc;
+        if (int rc = seam(Xn, w.n2w, w.n2b, h, UITK_T_MX4)) return rc;
+        if (int rc = linear(h, UITK_T_MX4, g.D, GEN_FC1, b, w.fc1_b, g.act_gelu ? 2 : 1, hid, UITK_T_MX4, g.hidden)) return rc;
+        if (int rc = linear(hid, UITK_T_MX4, g.hidden, GEN_FC2, b, w.fc2_b, 0, Xn, UITK_T_F32, g.D)) return rc;
+        const bool last = b + 1 == g.depth;
+        if (int rc = seam(Xn, last ? m->norm_w : m->blocks[b + 1].n1w, last ? m->norm_b : m->blocks[b + 1].n1b, last ? (void*)Xn : (void*)h, last ? UITK_T_F32 : UITK_T_MX4)) return rc;
+    }
     return UITK_OK;
 }
 
@@ -652,23 +740,20 @@ int uitk_general_encode(uitk_general* m, int64_t B, int64_t T, float* probs, flo
         GEN_HIP(hipGetLastError());
         GEN_HIP(launch_naive_linear(X0, m->pe_w, nullptr, R, (int)Mr, K, D, 0, 1, s));
         const int lnb = (int)((Mr + 3) / 4);
-        for (int b = 0; b < g.depth; ++b) {
+        if (m->mx4()) {
+            if (int rc = gen_blocks_mx4(m, g, n, R, Xn, QKV, O, scale, s)) return rc;
+        }
+        for (int b = 0; b < g.depth && !m->mx4(); ++b) {
             const GenBlockPtrs& w = m->blocks[b];
             hipLaunchKernelGGL(gen_layernorm_kernel, dim3(lnb), dim3(256), 0, s, R, Xn, w.n1w, w.n1b, Mr, D, 1e-6f);
             GEN_HIP(launch_naive_linear(Xn, w.qkv_w, w.qkv_b, QKV, (int)Mr, D, 3 * g.inner, 0, 0, s));
-            if (g.hd <= 8) gen_launch_attention<8>(QKV, O, n, g, g.ntok, scale, s);
-            else if (g.hd <= 16) gen_launch_attention<16>(QKV, O, n, g, g.ntok, scale, s);
-            else if (g.hd <= 32) gen_launch_attention<32>(QKV, O, n, g, g.ntok, scale, s);
-            else if (g.hd <= 64) gen_launch_attention<64>(QKV, O, n, g, g.ntok, scale, s);
-            else if (g.hd <= 128) gen_launch_attention<128>(QKV, O, n, g, g.ntok, scale, s);
-            else hipLaunchKernelGGL(gen_attention_wide_kernel, dim3(n * g.heads, (g.ntok + 63) / 64, (g.hd + 63) / 64), dim3(64), 0, s, QKV, O, g.ntok, g.heads, g.inner, g.hd, scale);
-            GEN_HIP(hipGetLastError());
+            GEN_HIP(gen_attention(QKV, O, n, g, scale, s));
             GEN_HIP(launch_naive_linear(O, w.proj_w, w.proj_b, R, (int)Mr, g.inner, D, 0, 1, s));
             hipLaunchKernelGGL(gen_layernorm_kernel, dim3(lnb), dim3(256), 0, s, R, Xn, w.n2w, w.n2b, Mr, D, 1e-6f);
             GEN_HIP(launch_naive_linear(Xn, w.fc1_w, w.fc1_b, Hd, (int)Mr, D, g.hidden, g.act_gelu ? 2 : 1, 0, s));
             GEN_HIP(launch_naive_linear(Hd, w.fc2_w, w.fc2_b, R, (int)Mr, g.hidden, D, 0, 1, s));
         }
-        hipLaunchKernelGGL(gen_layernorm_kernel, dim3(lnb), dim3(256), 0, s, R, Xn, m->norm_w, m->norm_b, Mr, D, 1e-6f);
+        if (!m->mx4()) hipLaunchKernelGGL(gen_layernorm_kernel, dim3(lnb), dim3(256), 0, s, R, Xn, m->norm_w, m->norm_b, Mr, D, 1e-6f);
         GenHeadArgs h{m->hln_w, m->hln_b, m->head_w, m->head_b, rowprobs + r0 * g.C, logits ? logits + r0 * g.C : nullptr};
         hipLaunchKernelGGL(gen_head_kernel, dim3(n), dim3(256), (size_t)D * 4, s, Xn, h, g);
         GEN_HIP(hipGetLastError());

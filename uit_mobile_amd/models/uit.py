@@ -32,12 +32,14 @@ _CALIB_OPTIONS = ('calib_accept_pct', 'calib_budget_e6', 'calib_short_check')   
 # 'fp8c' / 'fp8w' (round 5, BASELINE config #5): the fp8 kernel on weights GPTQ-rounded to the MX e4m3 grid / the f16 kernel on fp8-grid weights
 # ("fp8 weights" read literally), both calibrated like 'f16c'; 'fp8' keeps its weights rounded to nearest (the reference point)
 _PRECISIONS = {'auto': _lib.PREC_F16, 'f16': _lib.PREC_F16, 'f16c': _lib.PREC_F16, 'bf16': _lib.PREC_BF16, 'fp8': _lib.PREC_FP8, 'fp8c': _lib.PREC_FP8,
-               'fp8w': _lib.PREC_FP8W, 'f16x2': _lib.PREC_F16X2, 'f16l6': _lib.PREC_F16L6, 'f16a': _lib.PREC_F16A, 'f16ax': _lib.PREC_F16AX, 'f32': _lib.PREC_F32}
+               'fp8w': _lib.PREC_FP8W, 'f16x2': _lib.PREC_F16X2, 'f16l6': _lib.PREC_F16L6, 'f16a': _lib.PREC_F16A, 'f16ax': _lib.PREC_F16AX, 'f32': _lib.PREC_F32, 'mx4': _lib.PREC_MX4}
 _PRECISION_NAMES = {_lib.PREC_F16: 'f16', _lib.PREC_BF16: 'bf16', _lib.PREC_FP8: 'fp8', _lib.PREC_F16X2: 'f16x2', _lib.PREC_F16L6: 'f16l6', _lib.PREC_F16A: 'f16a', _lib.PREC_F16AX: 'f16ax', _lib.PREC_F32: 'f32'}
 # 'f16a' (round 5, pooling 'token' only): 'f16c' + the MLP's activation operands of the cls column tile as hi + lo terms -- what 'auto' escalates
 # to there (the cls row is read without a mean over tokens: activation rounding, not weight rounding, is what is over budget)
 _CALIBRATING = ('auto', 'f16c', 'fp8c', 'fp8w', 'f16a', 'f16ax')    # precisions whose handle is built with uitk_calibrate_weights
 # 'f16ax' (round 5): 'f16a' on the split weights of 'f16x2' -- where 'auto' goes when an 'f16a' handle is over the budget
+# 'mx4': the GENERAL engine's throughput mode -- the dense layers of its blocks on 4-bit weights and activations (mx4.py), the seams between them
+# in one kernel (norms.py), the rest fp32; for geometries outside the published factories', where the alternative is 'f32'
 # 'f32' (round 5): the plain fp32 forward of the library (vector ALUs; ~20x slower) -- the last rung of every ladder: where 'auto' ends when no
 # fp16 mode is inside the budget (checkpoints with strong attention sinks); any family, any pooling
 
@@ -219,12 +221,14 @@ class UITBase(nn.Module):
         if precision is not None and precision not in _PRECISIONS:
             raise ValueError(f"Unknown precision ({precision})")
         if self.general:
-            if precision not in (None, 'auto', 'f32'):
+            if precision not in (None, 'auto', 'f32', 'mx4'):
                 raise NotImplementedError(f"precision='{precision}' is an MFMA-kernel mode, built for the geometry of the published factories (embed 128, 2 heads, "
                                           "MLP x 3, 64 mels, n_fft 512, 16 x 16 patches, 6 time patches); this configuration runs on the general fp32 "
-                                          "engine: precision None / 'auto' / 'f32'")
-            precision = 'f32'
+                                          "engine: precision None / 'auto' / 'f32', or 'mx4' (its dense layers on 4-bit operands)")
+            precision = 'mx4' if precision == 'mx4' else 'f32'
             self.precision = precision
+        elif precision == 'mx4':
+            raise NotImplementedError("precision='mx4' is a mode of the general engine; this geometry runs on the MFMA encoder kernels, whose low-precision modes are 'fp8' / 'fp8c' / 'fp8w'")
         if precision is None:
             # default = THE PARITY MODE, for every family and pooling (round 5: 'auto').  It starts as 'f16c' -- single fp16 weights with
             # CALIBRATED rounding: the kernels of 'f16', the weights rounded against operand statistics (uitk_calibrate_weights) of the
@@ -243,7 +247,7 @@ class UITBase(nn.Module):
             raise NotImplementedError("precision='f16l6' is built for BNeckAttention + ReLU (any pooling)")
         if precision in ('f16a', 'f16ax') and pooling != 'token':
             raise NotImplementedError("precision='f16a' / 'f16ax' (split activation operands of the cls tile) are built for pooling='token'")
-        if pooling != 'mean' and precision not in ('auto', 'f16', 'f16c', 'f16l6', 'f16x2', 'fp8w', 'f16a', 'f16ax', 'f32'):
+        if pooling != 'mean' and precision not in ('auto', 'f16', 'f16c', 'f16l6', 'f16x2', 'fp8w', 'f16a', 'f16ax', 'f32', 'mx4'):
             raise NotImplementedError("pooling='dm' / 'token' are built for precision='auto' / 'f16' / 'f16c' / 'f16l6' / 'f16x2' / 'fp8w'")
 
         self.front_end = nn.Sequential(
@@ -506,7 +510,7 @@ class UITBase(nn.Module):
         if self.general:
             _lib.check(L.uitk_general_create(ctypes.byref(cfg), ctypes.byref(w), ctypes.byref(out)), "uitk_general_create")
             handle = _Handle(out.value, general=True)
-            handle.mode = {"precision": "f32", "requested": self.precision, "escalated": False, "reason": None, "check": None, "engine": "general"}
+            handle.mode = {"precision": self.precision, "requested": self.precision, "escalated": False, "reason": None, "check": None, "engine": "general"}
             return handle
         _lib.check(L.uitk_create(ctypes.byref(cfg), ctypes.byref(w), ctypes.byref(out)), "uitk_create")
         handle = _Handle(out.value)

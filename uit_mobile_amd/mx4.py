@@ -10,8 +10,9 @@ What `UITBase(precision='mx4')` runs its dense layers on (uit_mobile_amd/models/
 current stream; enqueue-only, safe inside a HIP graph capture.  No gradients: like the rest of this package these are inference operators,
 and a call that autograd would have to record is refused.
 """
-import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -19,33 +20,43 @@ from . import _lib
 
 _TYPES = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
 _ACTS = {None: 0, "relu": 1, "gelu": 2}
+_RECORD_BYTES, _MAX_ROWS, _MAX_K = 4096 + 256, 1 << 31, 1 << 20             # uitk_mx4_bytes, without the call
+_LINEAR_ARGS = struct.Struct("6Q6q4i")                                      # uitk_mx4_linear_args
+
+# A call for a single token is a few microseconds of GPU time, so what happens here before the launch is most of it: arguments travel as packed
+# bytes, a tensor is copied or converted only where it has to be, and the device is switched only where it is another one.
 
 
-def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+def run(fn, device, *args):
+    """Enqueue fn(*args, stream) on `device` and its current stream."""
+    i = device.index
+    stream = torch._C._cuda_getCurrentRawStream(i)
+    if torch._C._cuda_getDevice() == i:
+        return _lib.check(fn(*args, stream), fn.__name__)
+    with torch.cuda.device(i):
+        _lib.check(fn(*args, stream), fn.__name__)
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def check_tensor(t, name, dtypes=tuple(_TYPES)):
-    """A CUDA tensor of one of `dtypes` that needs no gradient (shared with norms.py)."""
+def check_tensor(t, name):
+    """A CUDA tensor of a type these operators take that needs no gradient -> its uitk_type (shared with norms.py)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor: uit_mobile_amd has no CPU path")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient: this is an inference operator (call it under torch.no_grad())")
+    return code
 
 
-def as_rows(t):
-    """[..., K] -> (tensor [rows, K] whose last dimension is contiguous, its row stride): a view where the strides allow, else a copy."""
-    K = t.shape[-1]
+def as_rows(t, K):
+    """[..., K] -> (a tensor that holds its rows, their distance in elements): `t` itself where its strides allow, else a copy."""
+    if t.is_contiguous():
+        return t, K
     rows = t.numel() // K if K else 0
-    v = t.view(rows, K) if t.is_contiguous() else t.reshape(rows, K)
+    v = t.reshape(rows, K)
     if K > 1 and v.stride(1) != 1 or rows > 1 and v.stride(0) < K:
         v = v.contiguous()
     return v, (v.stride(0) if rows > 1 else K)
@@ -63,15 +74,26 @@ def overlaps(a, b):
 
 
 def check_vector(t, name, n, device):
-    """A per-channel parameter: [n] on `device`, handed on in float32."""
+    """A per-channel parameter: [n] on `device` -> in float32, contiguous (None stays None)."""
     if t is None:
         return None
     check_tensor(t, name)
-    if t.shape != (n,):
+    if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    return t.detach().to(torch.float32).contiguous()
+    if t.dtype is not torch.float32:
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(M, N, K, x_type):
+    return _lib.load().uitk_mx4_linear_workspace(M, N, K, x_type)
 
 
 class Mx4Tensor:
@@ -85,10 +107,9 @@ class Mx4Tensor:
     @classmethod
     def empty(cls, shape, device):
         rows, K = math.prod(shape[:-1]), shape[-1]
-        n = _lib.load().uitk_mx4_bytes(rows, K)
-        if n < 0:
+        if rows > _MAX_ROWS or not 1 <= K <= _MAX_K:
             raise ValueError(f"a packed 4-bit matrix of {rows} rows x {K} is out of range (rows <= 2^31, 1 <= K <= 2^20)")
-        return cls(torch.empty(n, dtype=torch.uint8, device=device), shape)
+        return cls(torch.empty((rows + 63) // 64 * ((K + 127) // 128) * _RECORD_BYTES, dtype=torch.uint8, device=device), shape)
 
     @property
     def device(self):
@@ -110,23 +131,21 @@ class Mx4Tensor:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         if out.numel():
-            with torch.cuda.device(self.device):
-                _lib.check(_lib.load().uitk_mx4_dequantize(_ptr(self.data), self.rows, self.shape[-1], _ptr(out), _TYPES[dtype], self.shape[-1],
-                                                           _stream(self.device)), "uitk_mx4_dequantize")
+            K = self.shape[-1]
+            run(_lib.load().uitk_mx4_dequantize, out.device, self.data.data_ptr(), out.numel() // K, K, out.data_ptr(), _TYPES[dtype], K)
         return out
 
 
 def quantize(x):
     """x [..., K] (float32 / float16 / bfloat16) -> Mx4Tensor of the same shape."""
-    check_tensor(x, "x")
+    code = check_tensor(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., K] with K >= 1, got {tuple(x.shape)}")
     q = Mx4Tensor.empty(x.shape, x.device)
     if x.numel():
-        v, ld = as_rows(x.detach())
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.load().uitk_mx4_quantize(_ptr(v), _TYPES[v.dtype], v.shape[0], v.shape[1], ld, _ptr(q.data), _stream(x.device)),
-                       "uitk_mx4_quantize")
+        K = x.shape[-1]
+        v, ld = as_rows(x, K)
+        run(_lib.load().uitk_mx4_quantize, x.device, v.data_ptr(), code, x.numel() // K, K, ld, q.data.data_ptr())
     return q
 
 
@@ -138,63 +157,59 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
     Mx4Tensor, the next layer's x (no residual then).  out: write there instead (a contiguous tensor of the output's shape and type;
     `out=residual` accumulates in place)."""
     packed = isinstance(x, Mx4Tensor)
-    if not packed:
-        check_tensor(x, "x")
+    x_type = _lib.T_MX4 if packed else check_tensor(x, "x")
     if not isinstance(w, Mx4Tensor):
         raise TypeError("w must be an Mx4Tensor: quantize(weight) once")
     if len(w.shape) != 2:
         raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
-    if len(x.shape) < 1 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} does not match w {tuple(w.shape)}")
-    if w.device != x.device:
-        raise ValueError(f"w is on {w.device}, x on {x.device}")
+    N, K = w.shape
+    x_shape, device = x.shape, x.device
+    if len(x_shape) < 1 or x_shape[-1] != K:
+        raise ValueError(f"x {tuple(x_shape)} does not match w {tuple(w.shape)}")
+    if w.device != device:
+        raise ValueError(f"w is on {w.device}, x on {device}")
     if act not in _ACTS:
         raise ValueError(f"act must be None, 'relu' or 'gelu', got {act!r}")
-    device, (N, K) = x.device, w.shape
-    shape = tuple(x.shape[:-1]) + (N,)
-    M = math.prod(x.shape[:-1])
+    shape = x_shape[:-1] + (N,)
+    M = x.numel() // K
     if residual is not None:
         check_tensor(residual, "residual")
-    if out is not None and not isinstance(out, torch.Tensor):
-        raise TypeError("out must be a tensor")
+    if out is not None:
+        check_tensor(out, "out")
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.float32 if packed else x.dtype
     to_mx4 = out_dtype == "mx4"
     if not to_mx4 and out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16, bfloat16 or 'mx4', got {out_dtype}")
+    b = check_vector(bias, "bias", N, device)
+    res, ldr = None, 0
     if residual is not None:
         if to_mx4:
             raise ValueError("a residual needs an output of 16 or 32 bits")
         if residual.shape != shape or residual.dtype != out_dtype or residual.device != device:
-            raise ValueError(f"residual must be {shape} {out_dtype} on {device}, got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+            raise ValueError(f"residual must be {tuple(shape)} {out_dtype} on {device}, got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+        res, ldr = as_rows(residual, N)
     if out is not None:
         if to_mx4:
             raise ValueError("out is not supported for a 4-bit output")
-        check_tensor(out, "out")
-        if tuple(out.shape) != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {shape} {out_dtype} on {device}")
+        if out.shape != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {tuple(shape)} {out_dtype} on {device}")
         for name, t in (("x", x.data if packed else x), ("w", w.data), ("bias", bias)):
             if t is not None and overlaps(out, t):
                 raise ValueError(f"out shares memory with {name}")
         if residual is not None and overlaps(out, residual) and not (out.data_ptr() == residual.data_ptr() and residual.is_contiguous()):
             raise ValueError("out shares memory with the residual without being the residual")
-    b = check_vector(bias, "bias", N, device)
     if to_mx4:
         result = Mx4Tensor.empty(shape, device)
-        dst, ldo = result.data, 0
+        dst, out_type = result.data, _lib.T_MX4
     else:
         result = dst = torch.empty(shape, dtype=out_dtype, device=device) if out is None else out
-        ldo = N
+        out_type = _TYPES[out_dtype]
     if M == 0:
         return result
-    L = _lib.load()
-    x_type = _lib.T_MX4 if packed else _TYPES[x.dtype]
-    src, ldx = (x.data, 0) if packed else as_rows(x.detach())
-    res, ldr = (None, 0) if residual is None else as_rows(residual.detach())
-    need = L.uitk_mx4_linear_workspace(M, N, K, x_type)
+    src, ldx = (x.data, 0) if packed else as_rows(x, K)
+    need = _workspace_bytes(M, N, K, x_type)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    a = _lib.Mx4LinearArgs(x=_ptr(src), w=_ptr(w.data), bias=_ptr(b), residual=_ptr(res), out=_ptr(dst), workspace=_ptr(ws), M=M, N=N, K=K,
-                           ldx=ldx, ldr=ldr, ldo=ldo, x_type=x_type, out_type=_lib.T_MX4 if to_mx4 else _TYPES[out_dtype], act=_ACTS[act])
-    with torch.cuda.device(device):
-        _lib.check(L.uitk_mx4_linear(ctypes.byref(a), _stream(device)), "uitk_mx4_linear")
+    args = _LINEAR_ARGS.pack(src.data_ptr(), w.data.data_ptr(), ptr(b), ptr(res), dst.data_ptr(), ptr(ws), M, N, K, ldx, ldr, N, x_type, out_type, _ACTS[act], 0)
+    run(_lib.packed("uitk_mx4_linear"), device, args)
     return result
