@@ -101,7 +101,7 @@ struct Mx4LinearArgs {
     const void* residual; int64_t ldr;                                      // of the output's type, added last
     void* out; int64_t ldo; int out_type;                                   // MT_MX4: out = codes, out_scales its scales
     char* out_scales; int64_t out_S;
-    unsigned ngroups;                                                       // groups of 64 columns
+    unsigned ngroups;                                                       // column groups of the rows kernel
     int vec4;                                                               // every four-element group of bias / residual / out is aligned
 };
 
@@ -169,81 +169,85 @@ __device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, in
     else for (int i = 0; i < 4; ++i) if (n + i < a.N) o[i] = t[i];
 }
 
-// A workgroup computes 64 outputs (n) x 32 TT tokens (m); its waves take the records of K in turn, each with its own accumulators, and
-// join them through LDS in a fixed order.  Operands go from memory to registers in fragment order; activations that are not packed yet
-// are quantised by the lane that multiplies them (lane l of the B operand owns row l % 32, block l / 32: a whole block).
-template <int TT, typename XT>
-__device__ __forceinline__ void mx4_x_fragment(const Mx4LinearArgs& a, int64_t row, int64_t k, Mx4Block& b) {
-    b.codes = mx_i4{0, 0, 0, 0}; b.scale = 0;
+// ---- few rows, or few tiles: latency.  A workgroup computes 32 NT outputs (n) x 32 tokens (m); its NW waves take the records of K in turn, each
+// with its own accumulators, and join them through LDS in a fixed order.  Operands go from memory to registers in fragment order, a
+// record of weights ahead of its product; activations that are not packed yet are quantised by the lane that multiplies them (lane l of
+// the B operand owns row l % 32, block l / 32: a whole block).  Bound by reading the weights where there are many (13 x 8192 x 8192, packed x:
+// 11.9 us, 3.0 TB/s of weights), by the latency of a launch and one trip to memory where there are few (1 x 2304 x 768: 3.2 us).
+template <typename XT>
+__device__ __forceinline__ Mx4Block mx4_x_fragment(const Mx4LinearArgs& a, int64_t row, int64_t k) {
+    Mx4Block b{mx_i4{0, 0, 0, 0}, 0};
     if (row < a.M && k < a.K) {
         Mx4Src<XT> src;
         src.load((const XT*)a.x + row * a.ldx + k, a.x_vec, (int)min((int64_t)32, a.K - k));
         b = src.pack();
     }
+    return b;
 }
 
-template <int TT, typename XT, bool PACKED>
-__global__ void __launch_bounds__(256) mx4_linear_kernel(Mx4LinearArgs a) {
-    constexpr int NW = 4, LDT = 64 + 4;                                     // waves; floats per token row of the joining buffer
-    __shared__ __attribute__((aligned(16))) float red[NW][32 * TT][LDT];
+template <int NT, int NW, typename XT, bool PACKED>
+__global__ void __launch_bounds__(64 * NW) mx4_rows_kernel(Mx4LinearArgs a) {
+    constexpr int LDT = 32 * NT + 4;                                        // floats per token row of the joining buffer
+    extern __shared__ __attribute__((aligned(16))) float red[];             // [NW][32][LDT]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, g = lane >> 5;
-    const int64_t ng = blockIdx.x % a.ngroups, m0 = (int64_t)(blockIdx.x / a.ngroups) * 32 * TT;
-    mx_f16 acc[2][TT];
+    const int64_t nt = blockIdx.x % a.ngroups, m0 = (int64_t)(blockIdx.x / a.ngroups) * 32;
+    const int64_t ng = NT == 2 ? nt : nt >> 1;                              // the record's row group, and with NT = 1 the half of it
+    const int half = NT == 2 ? 0 : (int)(nt & 1);
+    mx_f16 acc[NT];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
+        for (int i = 0; i < 16; ++i) acc[rt][i] = 0.f;
+    mx_i4 wf[NT * 2];
+    int ws = 0;
+    auto weights = [&](int64_t s) {
+        const int64_t rec = ng * a.S + s;
+        const char* wc = a.w + rec * MX4_CODES + half * 2048 + lane * 16;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[rt][t][i] = 0.f;
-    const int64_t nrec_rows = (a.N + MX4_ROWS - 1) / MX4_ROWS;
-    if (ng < nrec_rows) {                                                   // (an out_type of 4 bits pads its columns to 128: such a group multiplies nothing)
+        for (int f = 0; f < NT * 2; ++f) wf[f] = *(const mx_i4*)(wc + f * 1024);
+        ws = *(const int*)(a.w_scales + rec * MX4_SCALES + lane * 4) >> (16 * half);
+    };
+    if (ng * MX4_ROWS + 32 * half < a.N && wave < a.S) {                    // (an out_type of 4 bits pads its columns to 128: such a group multiplies nothing)
+        weights(wave);
         for (int64_t s = wave; s < a.S; s += NW) {
-            const char* wc = a.w + (ng * a.S + s) * MX4_CODES;
-            const int ws = *(const int*)(a.w_scales + (ng * a.S + s) * MX4_SCALES + lane * 4);
-            mx_i4 wf[4];
+            mx_i4 w[NT * 2];
 #pragma unroll
-            for (int f = 0; f < 4; ++f) wf[f] = *(const mx_i4*)(wc + f * 1024 + lane * 16);
-#pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                if constexpr (PACKED) {
-                    const int64_t row = m0 + 32 * t;                        // a multiple of 32: row tile (row / 32) % 2 of its record
-                    if (row >= a.M) continue;
-                    const int64_t rec = (row >> 6) * a.S + s;
-                    const int rt = (int)(row >> 5) & 1;
-                    const int xs = *(const int*)(a.x_scales + rec * MX4_SCALES + lane * 4) >> (16 * rt);
-                    const char* xc = (const char*)a.x + rec * MX4_CODES + rt * 2048;
-                    const mx_i4 x0 = *(const mx_i4*)(xc + lane * 16), x1 = *(const mx_i4*)(xc + 1024 + lane * 16);
-                    acc[0][t] = mx4_mfma<0, 0>(wf[0], x0, acc[0][t], ws, xs);
-                    acc[1][t] = mx4_mfma<2, 0>(wf[2], x0, acc[1][t], ws, xs);
-                    acc[0][t] = mx4_mfma<1, 1>(wf[1], x1, acc[0][t], ws, xs);
-                    acc[1][t] = mx4_mfma<3, 1>(wf[3], x1, acc[1][t], ws, xs);
-                } else {
-                    Mx4Block x0, x1;
-                    mx4_x_fragment<TT, XT>(a, m0 + 32 * t + c, s * MX4_K + 32 * g, x0);
-                    mx4_x_fragment<TT, XT>(a, m0 + 32 * t + c, s * MX4_K + 64 + 32 * g, x1);
-                    acc[0][t] = mx4_mfma<0, 0>(wf[0], x0.codes, acc[0][t], ws, (int)x0.scale);
-                    acc[1][t] = mx4_mfma<2, 0>(wf[2], x0.codes, acc[1][t], ws, (int)x0.scale);
-                    acc[0][t] = mx4_mfma<1, 0>(wf[1], x1.codes, acc[0][t], ws, (int)x1.scale);
-                    acc[1][t] = mx4_mfma<3, 0>(wf[3], x1.codes, acc[1][t], ws, (int)x1.scale);
-                }
+            for (int f = 0; f < NT * 2; ++f) w[f] = wf[f];
+            const int wsc = ws;
+            if (s + NW < a.S) weights(s + NW);
+            Mx4Block x0, x1;                                                // the two halves of the record; their scales in bytes 0 and 1 where packed
+            if constexpr (PACKED) {
+                const int64_t rec = (m0 >> 6) * a.S + s;
+                const int rt = (int)(m0 >> 5) & 1;
+                const char* xc = (const char*)a.x + rec * MX4_CODES + rt * 2048 + lane * 16;
+                x0.codes = *(const mx_i4*)xc;
+                x1.codes = *(const mx_i4*)(xc + 1024);
+                x0.scale = x1.scale = *(const unsigned*)(a.x_scales + rec * MX4_SCALES + lane * 4) >> (16 * rt);
+            } else {
+                x0 = mx4_x_fragment<XT>(a, m0 + c, s * MX4_K + 32 * g);
+                x1 = mx4_x_fragment<XT>(a, m0 + c, s * MX4_K + 64 + 32 * g);
             }
+            acc[0] = mx4_mfma<0, 0>(w[0], x0.codes, acc[0], wsc, (int)x0.scale);
+            if constexpr (NT == 2) acc[1] = mx4_mfma<2, 0>(w[2], x0.codes, acc[1], wsc, (int)x0.scale);
+            acc[0] = mx4_mfma<1, PACKED ? 1 : 0>(w[1], x1.codes, acc[0], wsc, (int)x1.scale);
+            if constexpr (NT == 2) acc[1] = mx4_mfma<3, PACKED ? 1 : 0>(w[3], x1.codes, acc[1], wsc, (int)x1.scale);
         }
     }
+    float* mine = red + wave * 32 * LDT;
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *(mx_f4*)&red[wave][32 * t + c][32 * rt + 8 * q + 4 * g] = mx_f4{acc[rt][t][4 * q], acc[rt][t][4 * q + 1], acc[rt][t][4 * q + 2], acc[rt][t][4 * q + 3]};
+        for (int q = 0; q < 4; ++q) *(mx_f4*)&mine[c * LDT + 32 * rt + 8 * q + 4 * g] = mx_f4{acc[rt][4 * q], acc[rt][4 * q + 1], acc[rt][4 * q + 2], acc[rt][4 * q + 3]};
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * TT * 16; i += 256) {
-        const int t = i >> 4, n4 = (i & 15) * 4;
-        mx_f4 s = *(const mx_f4*)&red[0][t][n4];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) s += *(const mx_f4*)&red[w][t][n4];
+    const int nw = (int)min((int64_t)NW, a.S);                              // (the other waves had no record)
+    for (int i = threadIdx.x; i < 32 * 8 * NT; i += 64 * NW) {              // (whole waves: the 4-bit store exchanges maxima between lanes)
+        const int t = i / (8 * NT), n4 = i % (8 * NT) * 4;
+        const float* p = red + t * LDT + n4;
+        mx_f4 s = *(const mx_f4*)p;
+        for (int w = 1; w < nw; ++w) s += *(const mx_f4*)(p + w * 32 * LDT);
         float v[4] = {s[0], s[1], s[2], s[3]};
-        mx4_store4(a, m0 + t, ng * 64 + n4, mx4_bias4(a, ng * 64 + n4), v);
+        const int64_t n = nt * 32 * NT + n4;
+        mx4_store4(a, m0 + t, n, mx4_bias4(a, n), v);
     }
 }
 
@@ -319,23 +323,32 @@ __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const flo
     const int lane = threadIdx.x & 63;
     constexpr int LPR = COLS / 4, RPI = 64 / LPR;                           // lanes that hold a row, rows an instruction stores
     if constexpr (OUT == MT_MX4) {
-        const int64_t n = n0 + (lane % LPR) * 4;
-        if (n0 >= a.out_S * MX4_K) return;
-        const mx_f4 bias = mx4_bias4(a, n);
+        // eight columns a lane, four lanes a block; m0 is a multiple of 32, so a lane's blocks lie 16 bytes a row apart
+        constexpr int L8 = COLS / 8, R8 = 64 / L8;
+        const int64_t n = n0 + (lane % L8) * 8;
+        if (n0 >= a.out_S * MX4_K || m0 >= a.M) return;
+        const mx_f4 b0 = mx4_bias4(a, n), b1 = mx4_bias4(a, n + 4);
         const bool inside = n0 + COLS <= a.N;
-#pragma unroll 4
-        for (int it = 0; it < 32 / RPI; ++it) {
-            const int t = it * RPI + lane / LPR;
-            const mx_f4 w = *(const mx_f4*)&ep[t * LDE + (lane % LPR) * 4];
-            float v[4];
+        const Mx4Place p = mx4_place(m0 + lane / L8, n >> 5, a.out_S);
+        char* code = (char*)a.out + p.code + ((n & 31) >> 1);
+        char* scale = a.out_scales + p.scale;
+        const int rows = (int)min((int64_t)32, a.M - m0);
+#pragma unroll 2
+        for (int it = 0; it < 32 / R8; ++it) {
+            const int t = it * R8 + lane / L8;
+            const mx_f4 w0 = *(const mx_f4*)&ep[t * LDE + (lane % L8) * 8], w1 = *(const mx_f4*)&ep[t * LDE + (lane % L8) * 8 + 4];
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = mx4_act<ACT>(w[i] + bias[i]); if (!inside && n + i >= a.N) v[i] = 0.f; }
+            for (int i = 0; i < 4; ++i) { v[i] = mx4_act<ACT>(w0[i] + b0[i]); v[4 + i] = mx4_act<ACT>(w1[i] + b1[i]); }
+            if (!inside) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) if (n + i >= a.N) v[i] = 0.f;
+            }
             unsigned sc;
-            const unsigned two = mx4_pack_quads(v, &sc);                    // (every lane is here: the 8 lanes of a block exchange their maxima)
-            if (m0 + t < a.M) {
-                const Mx4Place p = mx4_place(m0 + t, n >> 5, a.out_S);
-                *(unsigned short*)((char*)a.out + p.code + ((n & 31) >> 1)) = (unsigned short)two;
-                if ((n & 31) == 0) a.out_scales[p.scale] = (char)sc;
+            const unsigned four = mx4_pack_octets(v, &sc);                  // (every lane is here: the 4 lanes of a block exchange their maxima)
+            if (t < rows) {
+                *(unsigned*)(code + it * R8 * 16) = four;
+                if ((n & 31) == 0) scale[it * R8 * 4] = (char)sc;
             }
         }
     } else {
@@ -531,22 +544,45 @@ static int mx4_check_matrix(const char* what, int64_t rows, int64_t K) {
 static int type_size(int t) { return t == UITK_T_F32 ? 4 : 2; }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int TT>
-static void mx4_launch_linear(dim3 grid, const Mx4LinearArgs& a, hipStream_t s) {
-    if (a.x_type == MT_MX4) hipLaunchKernelGGL((mx4_linear_kernel<TT, float, true>), grid, dim3(256), 0, s, a);
-    else if (a.x_type == MT_F32) hipLaunchKernelGGL((mx4_linear_kernel<TT, float, false>), grid, dim3(256), 0, s, a);
-    else if (a.x_type == MT_F16) hipLaunchKernelGGL((mx4_linear_kernel<TT, _Float16, false>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((mx4_linear_kernel<TT, __bf16, false>), grid, dim3(256), 0, s, a);
+template <int NT, int NW>
+static hipError_t mx4_launch_rows(Mx4LinearArgs& a, hipStream_t s) {
+    const int64_t cols = a.out_type == MT_MX4 ? a.out_S * MX4_K : a.N;
+    const int64_t ngroups = (cols + 32 * NT - 1) / (32 * NT), mt = (a.M + 31) / 32;
+    if (mt * ngroups > ((int64_t)1 << 32) / (64 * NW) - 1) return hipErrorInvalidConfiguration;
+    a.ngroups = (unsigned)ngroups;
+    const dim3 grid((unsigned)(mt * ngroups));
+    constexpr int lds = NW * 32 * (32 * NT + 4) * 4;
+    auto go = [&](auto kernel) {
+        if (lds > 64 * 1024)                                                // (of the current device: set at every call, not once per process)
+            if (hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds); e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * NW), lds, s, a);
+        return hipGetLastError();
+    };
+    if (a.x_type == MT_MX4) return go(mx4_rows_kernel<NT, NW, float, true>);
+    if (a.x_type == MT_F32) return go(mx4_rows_kernel<NT, NW, float, false>);
+    if (a.x_type == MT_F16) return go(mx4_rows_kernel<NT, NW, _Float16, false>);
+    return go(mx4_rows_kernel<NT, NW, __bf16, false>);
 }
 
-enum { MX4_SMALL = 0, MX4_TILE128 = 1, MX4_TILE256 = 2 };
-// Which kernel: few rows (or few tiles) are a matter of latency; the wide tile needs two workgroups on every CU, and a K long enough that its
-// longer epilogue does not matter (us, small / 128 x 128 / 256 x 128 tile: 1024 x 1024 x 1024: 7.0 / 7.7 / 17; 2048 x 2048 x 2048: 17.2 / 12.3 / 17;
-// 16128 x 2304 x 768: 112 / 32.8 / 38.1; 4096 x 4096 x 4096: 95 / 47.2 / 41.9; 8192 x 8192 x 8192: 658 / 304 / 281).
-static int mx4_choose(int64_t M, int64_t N, int64_t K) {
-    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128), t256 = ((M + 127) / 128) * ((N + 255) / 256);
-    if (M <= 64 || t128 <= 64) return MX4_SMALL;
-    return t256 >= 512 && K >= 2048 ? MX4_TILE256 : MX4_TILE128;
+// Which kernel, and whether activations that are not packed are quantised inside it.  us on the GPU, launches back to back in a graph:
+// * rows against tiles: 128 x 128 tiles need more than 128 of them (packed x; rows / 128 x 128 / 256 x 128: 256 x 8192 x 8192: 20 / 26 / 41;
+//   512 x 4096 x 4096: 15 / 16 / 24; 2048 x 2048 x 2048: 17 / 12 / 17), the wide ones two workgroups on every CU and a K that outweighs
+//   their longer epilogue (16128 x 2304 x 768: - / 33 / 38; 4096 x 4096 x 4096: 95 / 47 / 42; 8192 x 8192 x 8192: 658 / 304 / 281).
+// * rows: 8 waves share K, 16 where a wave would still have two records or more (13 x 8192 x 8192, 8 / 16: 12.5 / 11.9); with more than 512
+//   workgroups 64 columns each instead of 32 (128 x 8192 x 8192, 32 / 64: 21.4 / 17.5).
+// * quantising inside repeats the work in every column group, about 65 vector instructions per 32 x 64 fragment, and costs more than a
+//   launch of its own (2.6 us) from 4096 fragments on: inside / packed: 1 x 2304 x 768 (864 fragments) 4.4 / 3.2, 252 x 768 x 768 (2304) 4.9 / 3.4,
+//   252 x 2304 x 768 (6912) 7.4 / 4.1, 13 x 8192 x 8192 (32768) 17.7 / 11.9.
+enum { MX4_ROWS8 = 0, MX4_ROWS16, MX4_ROWS64, MX4_TILE128, MX4_TILE256 };
+struct Mx4Plan { int kernel; bool quantize_first; };
+static Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t K, int x_type) {
+    const int64_t m128 = (M + 127) / 128, S = (K + MX4_K - 1) / MX4_K, groups = ((N + 31) / 32) * ((M + 31) / 32);
+    Mx4Plan p{MX4_ROWS8, x_type != MT_MX4};
+    if (M > 64 && m128 * ((N + 127) / 128) > 128) p.kernel = m128 * ((N + 255) / 256) >= 512 && K >= 2048 ? MX4_TILE256 : MX4_TILE128;
+    else if (groups > 512) p.kernel = MX4_ROWS64;
+    else if (S >= 32) p.kernel = MX4_ROWS16;
+    if (p.kernel < MX4_TILE128 && 2 * groups * S <= 4096) p.quantize_first = false;
+    return p;
 }
 
 template <int BN, int BM, int WN, int WM, int OUT>
@@ -620,8 +656,7 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
 
 int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type) {
     if (M < 0 || M > MX4_MAX_ROWS || N < 1 || N > MX4_MAX_K || K < 1 || K > MX4_MAX_K || x_type < UITK_T_F32 || x_type > UITK_T_MX4) return -1;
-    // activations that are not packed: the tile kernels read them from a packed copy, the others quantise as they go
-    return x_type != UITK_T_MX4 && mx4_choose(M, N, K) != MX4_SMALL ? mx4_bytes(M, K) : 0;
+    return mx4_plan(M, N, K, x_type).quantize_first ? mx4_bytes(M, K) : 0;
 }
 
 int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
@@ -653,31 +688,19 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
         a.vec4 = (uintptr_t)u->out % grp == 0 && u->ldo % 4 == 0 && (!u->residual || ((uintptr_t)u->residual % grp == 0 && u->ldr % 4 == 0));
     }
     hipStream_t s = (hipStream_t)stream;
-#ifdef UITK_LAB
-    const int kind = u->reserved ? u->reserved - 1 : mx4_choose(u->M, u->N, u->K);
-#else
-    const int kind = mx4_choose(u->M, u->N, u->K);
-#endif
-    if (kind == MX4_SMALL) {
-        const int64_t ngroups = u->out_type == UITK_T_MX4 ? 2 * a.out_S : (u->N + MX4_ROWS - 1) / MX4_ROWS;
-        const int tt = u->M <= 32 ? 1 : 2;
-        const int64_t mt = (u->M + 32 * tt - 1) / (32 * tt);
-        if (mt * ngroups > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
-        a.ngroups = (unsigned)ngroups;
-        const dim3 grid((unsigned)(mt * ngroups));
-        if (tt == 1) mx4_launch_linear<1>(grid, a, s); else mx4_launch_linear<2>(grid, a, s);
-    } else {
-        if (u->x_type != UITK_T_MX4) {
-            if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
-            if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
-            a.x = u->workspace; a.x_type = MT_MX4; a.x_scales = (const char*)u->workspace + mx4_records(u->M, u->K) * MX4_CODES;
-        }
-        const hipError_t e = kind == MX4_TILE256 ? mx4_launch_tile<256, 128, 2, 2>(a, s) : mx4_launch_tile<128, 128, 2, 2>(a, s);
-        if (e == hipErrorInvalidConfiguration) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
-        MX4_HIP(e);
-        return UITK_OK;
+    const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
+    if (plan.quantize_first) {
+        if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
+        if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
+        a.x = u->workspace; a.x_type = MT_MX4; a.x_scales = (const char*)u->workspace + mx4_records(u->M, u->K) * MX4_CODES;
     }
-    MX4_HIP(hipGetLastError());
+    const hipError_t e = plan.kernel == MX4_TILE256   ? mx4_launch_tile<256, 128, 2, 2>(a, s)
+                         : plan.kernel == MX4_TILE128 ? mx4_launch_tile<128, 128, 2, 2>(a, s)
+                         : plan.kernel == MX4_ROWS64  ? mx4_launch_rows<2, 8>(a, s)
+                         : plan.kernel == MX4_ROWS16  ? mx4_launch_rows<1, 16>(a, s)
+                                                      : mx4_launch_rows<1, 8>(a, s);
+    if (e == hipErrorInvalidConfiguration) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
+    MX4_HIP(e);
     return UITK_OK;
 }
 
