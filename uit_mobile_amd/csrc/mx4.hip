@@ -22,7 +22,7 @@ int set_error(int code, const std::string& msg);                          // api
 // One wave per record: lane (r = l % 32, g = l / 32) owns the blocks (row 32 rt + r, elements 64 kh + 32 g ..) of the four fragments,
 // so the maximum, the scale and the 16 bytes of a block never leave the lane, and a wave writes whole contiguous fragments.
 template <typename T>
-__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K, int64_t ld, int vec, int64_t R, int64_t S,
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K, int64_t ld, int64_t R, int64_t S,
                                                            char* __restrict__ codes, char* __restrict__ scales) {
     const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
     const int64_t rec = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
         Mx4Block b{mx_i4{0, 0, 0, 0}, 0};
         if (row < rows && k < K) {
             Mx4Src<T> src;
-            src.load(x + row * ld + k, vec, (int)min((int64_t)32, K - k));
+            src.load(x + row * ld + k, (int)min((int64_t)32, K - k));
             b = src.pack();
         }
         *(mx_i4*)(codes + rec * MX4_CODES + f * 1024 + lane * 16) = b.codes;
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
 
 // One wave per record here too, but 16 lanes share a row: each turns four bytes of codes into eight elements, so that a wave stores 128
 // consecutive elements of four rows at a time (a whole block per lane would store 16-byte pieces 64 bytes apart).
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales, int64_t rows, int64_t K, int64_t ld,
                                                              int64_t R, int64_t S, T* __restrict__ x) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, kb = l16 >> 2;      // the lane's block of its row: half kb / 2, group kb % 2
@@ -73,15 +73,16 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restr
         }
         if (row >= rows || n <= 0) continue;
         T* o = x + row * ld + k;
-        if (VEC && n == 8) {
+        if (n == 8) {
             typedef T T8 __attribute__((ext_vector_type(16 / sizeof(T))));
+            typedef T T8u __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
             constexpr int P = 16 / sizeof(T);                               // elements of a 16-byte store
 #pragma unroll
             for (int h = 0; h < 8 / P; ++h) {
                 T8 t;
 #pragma unroll
                 for (int i = 0; i < P; ++i) t[i] = (T)v[h * P + i];
-                *(T8*)(o + h * P) = t;
+                *(T8u*)(o + h * P) = t;
             }
         } else {
 #pragma unroll
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restr
 
 // --------------------------------------------------------------------------------------------------------------------- linear
 struct Mx4LinearArgs {
-    const void* x; int64_t M, K, ldx; int x_type, x_vec;                    // x_type MT_MX4: x = codes of a packed matrix, x_scales its scales
+    const void* x; int64_t M, K, ldx; int x_type;                           // x_type MT_MX4: x = codes of a packed matrix, x_scales its scales
     const char* x_scales;
     const char* w; const char* w_scales;                                    // packed [N, K]
     int64_t N, S;                                                           // S = records along K
@@ -102,16 +103,62 @@ struct Mx4LinearArgs {
     void* out; int64_t ldo; int out_type;                                   // MT_MX4: out = codes, out_scales its scales
     char* out_scales; int64_t out_S;
     unsigned ngroups;                                                       // column groups of the rows kernel
-    int vec4;                                                               // every four-element group of bias / residual / out is aligned
 };
 
 __device__ __forceinline__ mx_f4 mx4_bias4(const Mx4LinearArgs& a, int64_t n) {
     mx_f4 b = {0.f, 0.f, 0.f, 0.f};
-    if (a.bias) {
+    if (a.bias && n + 4 <= a.N) b = *(const mx_f4u*)(a.bias + n);
+    else if (a.bias) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (n + i < a.N) b[i] = a.bias[n + i];
     }
     return b;
+}
+
+// four consecutive outputs of a type: add a residual, round once, store
+template <int OUT> struct Mx4Out;
+template <> struct Mx4Out<MT_F32> {
+    typedef float T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const float* r) { const mx_f4 t = *(const mx_f4u*)r; v[0] += t[0]; v[1] += t[1]; v[2] += t[2]; v[3] += t[3]; }
+    static __device__ __forceinline__ void put4(float* o, const float (&v)[4]) { *(mx_f4u*)o = mx_f4{v[0], v[1], v[2], v[3]}; }
+};
+template <> struct Mx4Out<MT_F16> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const _Float16* r) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));            // (a bit cast of ONE element of a vector reads element 0, whichever was named)
+        const h4 t = *(const h4*)r;
+        v[0] += (float)t[0]; v[1] += (float)t[1]; v[2] += (float)t[2]; v[3] += (float)t[3];
+    }
+    static __device__ __forceinline__ void put4(_Float16* o, const float (&v)[4]) {
+        const mx_h2 a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
+        *(mx_u2u*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    }
+};
+template <> struct Mx4Out<MT_BF16> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ void add4(float (&v)[4], const __bf16* r) {
+        const mx_u2 t = *(const mx_u2u*)r;
+        v[0] += __uint_as_float(t[0] << 16); v[1] += __uint_as_float(t[0] & 0xffff0000u); v[2] += __uint_as_float(t[1] << 16); v[3] += __uint_as_float(t[1] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void put4(__bf16* o, const float (&v)[4]) {
+        const mx_b2 a = {(__bf16)v[0], (__bf16)v[1]}, b = {(__bf16)v[2], (__bf16)v[3]};
+        *(mx_u2u*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    }
+};
+// n of the four are inside the row
+template <int OUT>
+__device__ __forceinline__ void mx4_finish4(void* out, int64_t o, const void* residual, int64_t r, int n, float (&v)[4]) {
+    typedef typename Mx4Out<OUT>::T T;
+    T* po = (T*)out + o;
+    const T* pr = residual ? (const T*)residual + r : nullptr;
+    if (n >= 4) {
+        if (pr) Mx4Out<OUT>::add4(v, pr);
+        Mx4Out<OUT>::put4(po, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) po[i] = (T)(pr ? v[i] + (float)pr[i] : v[i]);
+    }
 }
 
 // four consecutive outputs (row m, columns n ..): bias, activation, residual, one rounding, store
@@ -135,38 +182,10 @@ __device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, in
         return;
     }
     if (!in_m || n >= a.N) return;
-    const bool four = a.vec4 && n + 4 <= a.N;
-    if (a.out_type == MT_F32) {
-        float* o = (float*)a.out + m * a.ldo + n;
-        const float* r = a.residual ? (const float*)a.residual + m * a.ldr + n : nullptr;
-        if (four) {
-            mx_f4 t = {v[0], v[1], v[2], v[3]};
-            if (r) t += *(const mx_f4*)r;
-            *(mx_f4*)o = t;
-        } else {
-            for (int i = 0; i < 4; ++i) if (n + i < a.N) o[i] = r ? r[i] + v[i] : v[i];
-        }
-        return;
-    }
-    unsigned short* o = (unsigned short*)a.out + m * a.ldo + n;
-    const unsigned short* r = a.residual ? (const unsigned short*)a.residual + m * a.ldr + n : nullptr;
-    unsigned short t[4] = {0, 0, 0, 0};
-    if (r) {
-        if (four) { const mx_u2 u = *(const mx_u2*)r; t[0] = (unsigned short)u[0]; t[1] = (unsigned short)(u[0] >> 16); t[2] = (unsigned short)u[1]; t[3] = (unsigned short)(u[1] >> 16); }
-        else for (int i = 0; i < 4; ++i) if (n + i < a.N) t[i] = r[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (a.out_type == MT_F16) {
-            if (r) v[i] += (float)__builtin_bit_cast(_Float16, t[i]);
-            t[i] = __builtin_bit_cast(unsigned short, (_Float16)v[i]);
-        } else {
-            if (r) v[i] += __uint_as_float((unsigned)t[i] << 16);
-            t[i] = __builtin_bit_cast(unsigned short, (__bf16)v[i]);
-        }
-    }
-    if (four) *(mx_u2*)o = mx_u2{(unsigned)t[0] | (unsigned)t[1] << 16, (unsigned)t[2] | (unsigned)t[3] << 16};
-    else for (int i = 0; i < 4; ++i) if (n + i < a.N) o[i] = t[i];
+    const int in = (int)min((int64_t)4, a.N - n);
+    if (a.out_type == MT_F32) mx4_finish4<MT_F32>(a.out, m * a.ldo + n, a.residual, m * a.ldr + n, in, v);
+    else if (a.out_type == MT_F16) mx4_finish4<MT_F16>(a.out, m * a.ldo + n, a.residual, m * a.ldr + n, in, v);
+    else mx4_finish4<MT_BF16>(a.out, m * a.ldo + n, a.residual, m * a.ldr + n, in, v);
 }
 
 // ---- few rows, or few tiles: latency.  A workgroup computes 32 NT outputs (n) x 32 tokens (m); its NW waves take the records of K in turn, each
@@ -179,7 +198,7 @@ __device__ __forceinline__ Mx4Block mx4_x_fragment(const Mx4LinearArgs& a, int64
     Mx4Block b{mx_i4{0, 0, 0, 0}, 0};
     if (row < a.M && k < a.K) {
         Mx4Src<XT> src;
-        src.load((const XT*)a.x + row * a.ldx + k, a.x_vec, (int)min((int64_t)32, a.K - k));
+        src.load((const XT*)a.x + row * a.ldx + k, (int)min((int64_t)32, a.K - k));
         b = src.pack();
     }
     return b;
@@ -281,37 +300,7 @@ struct Mx4Tile {
 };
 
 // ---- a wave's 32 tokens x 32 TN outputs, from its part of LDS to memory.  n0, m0: the first column / row; bias added, activation, residual
-// added, one rounding.  Whole tiles of aligned rows go four columns a lane; what sticks out or is not aligned goes one column a lane.
-template <int OUT> struct Mx4Out;
-template <> struct Mx4Out<MT_F32> {
-    typedef float T;
-    static __device__ __forceinline__ void add4(float (&v)[4], const float* r) { const mx_f4 t = *(const mx_f4*)r; v[0] += t[0]; v[1] += t[1]; v[2] += t[2]; v[3] += t[3]; }
-    static __device__ __forceinline__ void put4(float* o, const float (&v)[4]) { *(mx_f4*)o = mx_f4{v[0], v[1], v[2], v[3]}; }
-};
-template <> struct Mx4Out<MT_F16> {
-    typedef _Float16 T;
-    static __device__ __forceinline__ void add4(float (&v)[4], const _Float16* r) {
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));            // (a bit cast of ONE element of a vector reads element 0, whichever was named)
-        const h4 t = *(const h4*)r;
-        v[0] += (float)t[0]; v[1] += (float)t[1]; v[2] += (float)t[2]; v[3] += (float)t[3];
-    }
-    static __device__ __forceinline__ void put4(_Float16* o, const float (&v)[4]) {
-        const mx_h2 a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
-        *(mx_u2*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
-    }
-};
-template <> struct Mx4Out<MT_BF16> {
-    typedef __bf16 T;
-    static __device__ __forceinline__ void add4(float (&v)[4], const __bf16* r) {
-        const mx_u2 t = *(const mx_u2*)r;
-        v[0] += __uint_as_float(t[0] << 16); v[1] += __uint_as_float(t[0] & 0xffff0000u); v[2] += __uint_as_float(t[1] << 16); v[3] += __uint_as_float(t[1] & 0xffff0000u);
-    }
-    static __device__ __forceinline__ void put4(__bf16* o, const float (&v)[4]) {
-        const mx_b2 a = {(__bf16)v[0], (__bf16)v[1]}, b = {(__bf16)v[2], (__bf16)v[3]};
-        *(mx_u2*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
-    }
-};
-
+// added, one rounding, four columns a lane.
 template <int ACT> __device__ __forceinline__ float mx4_act(float v) {
     if constexpr (ACT == 1) return v < 0.f ? 0.f : v;                       // (a NaN stays one)
     else if constexpr (ACT == 2) return mx4_gelu(v);
@@ -354,34 +343,23 @@ __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const flo
     } else {
         typedef typename Mx4Out<OUT>::T T;
         if (m0 >= a.M || n0 >= a.N) return;
-        if (a.vec4 && n0 + COLS <= a.N && m0 + 32 <= a.M) {
-            const int64_t n = n0 + (lane % LPR) * 4;
-            const mx_f4 bias = mx4_bias4(a, n);
-            T* o = (T*)a.out + (m0 + lane / LPR) * a.ldo + n;
-            const T* r = a.residual ? (const T*)a.residual + (m0 + lane / LPR) * a.ldr + n : nullptr;
+        const int64_t n = n0 + (lane % LPR) * 4;
+        const mx_f4 bias = mx4_bias4(a, n);
+        const int row = lane / LPR, in = (int)min((int64_t)4, a.N - n);
+        int64_t o = (m0 + row) * a.ldo + n, r = (m0 + row) * a.ldr + n;
+        const bool whole = n0 + COLS <= a.N && m0 + 32 <= a.M;              // (of the wave)
+        const int rows = (int)min((int64_t)32, a.M - m0);
 #pragma unroll 4
-            for (int it = 0; it < 32 / RPI; ++it) {
-                const mx_f4 w = *(const mx_f4*)&ep[(it * RPI + lane / LPR) * LDE + (lane % LPR) * 4];
-                float v[4];
+        for (int it = 0; it < 32 / RPI; ++it, o += RPI * a.ldo, r += RPI * a.ldr) {
+            const mx_f4 w = *(const mx_f4*)&ep[(it * RPI + row) * LDE + (lane % LPR) * 4];
+            float v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = mx4_act<ACT>(w[i] + bias[i]);
-                if (r) Mx4Out<OUT>::add4(v, r + it * RPI * a.ldr);
-                Mx4Out<OUT>::put4(o + it * RPI * a.ldo, v);
-            }
-        } else {
-            const int rows = (int)min((int64_t)32, a.M - m0);
-#pragma unroll
-            for (int c = 0; c < COLS / 64; ++c) {
-                const int64_t n = n0 + c * 64 + lane;
-                if (n >= a.N) continue;
-                const float bias = a.bias ? a.bias[n] : 0.f;
-                T* o = (T*)a.out + m0 * a.ldo + n;
-                const T* r = a.residual ? (const T*)a.residual + m0 * a.ldr + n : nullptr;
-                for (int t = 0; t < rows; ++t) {
-                    float v = mx4_act<ACT>(ep[t * LDE + c * 64 + lane] + bias);
-                    if (r) v += (float)r[t * a.ldr];
-                    o[t * a.ldo] = (T)v;
-                }
+            for (int i = 0; i < 4; ++i) v[i] = mx4_act<ACT>(w[i] + bias[i]);
+            if (whole) {
+                if (a.residual) Mx4Out<OUT>::add4(v, (const T*)a.residual + r);
+                Mx4Out<OUT>::put4((T*)a.out + o, v);
+            } else if (it * RPI + row < rows && in > 0) {
+                mx4_finish4<OUT>(a.out, o, a.residual, r, in, v);
             }
         }
     }
@@ -541,7 +519,6 @@ static int mx4_check_matrix(const char* what, int64_t rows, int64_t K) {
     if (K < 1 || K > MX4_MAX_K) return set_error(UITK_ERR_INVALID_ARG, std::string(what) + ": the width must be 1 .. 2^20");
     return UITK_OK;
 }
-static int type_size(int t) { return t == UITK_T_F32 ? 4 : 2; }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <int NT, int NW>
@@ -621,13 +598,12 @@ int uitk_mx4_quantize(const void* x, int type, int64_t rows, int64_t K, int64_t 
     const int64_t R = (rows + MX4_ROWS - 1) / MX4_ROWS, S = (K + MX4_K - 1) / MX4_K;
     char* codes = (char*)q;
     char* scales = codes + R * S * MX4_CODES;
-    const int vec = aligned16(x) && (ld * type_size(type)) % 16 == 0;
     if ((R * S + 3) / 4 > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_quantize: more elements than one launch takes");
     const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_quantize_kernel<float>, grid, block, 0, s, (const float*)x, rows, K, ld, vec, R, S, codes, scales);
-    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_quantize_kernel<_Float16>, grid, block, 0, s, (const _Float16*)x, rows, K, ld, vec, R, S, codes, scales);
-    else hipLaunchKernelGGL(mx4_quantize_kernel<__bf16>, grid, block, 0, s, (const __bf16*)x, rows, K, ld, vec, R, S, codes, scales);
+    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_quantize_kernel<float>, grid, block, 0, s, (const float*)x, rows, K, ld, R, S, codes, scales);
+    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_quantize_kernel<_Float16>, grid, block, 0, s, (const _Float16*)x, rows, K, ld, R, S, codes, scales);
+    else hipLaunchKernelGGL(mx4_quantize_kernel<__bf16>, grid, block, 0, s, (const __bf16*)x, rows, K, ld, R, S, codes, scales);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }
@@ -645,11 +621,9 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     const char* scales = codes + R * S * MX4_CODES;
     const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    const bool vec = aligned16(x) && (ld * type_size(type)) % 16 == 0;
-    auto launch = [&](auto kernel, auto* out) { hipLaunchKernelGGL(kernel, grid, block, 0, s, codes, scales, rows, K, ld, R, S, out); };
-    if (type == UITK_T_F32) vec ? launch(mx4_dequantize_kernel<float, true>, (float*)x) : launch(mx4_dequantize_kernel<float, false>, (float*)x);
-    else if (type == UITK_T_F16) vec ? launch(mx4_dequantize_kernel<_Float16, true>, (_Float16*)x) : launch(mx4_dequantize_kernel<_Float16, false>, (_Float16*)x);
-    else vec ? launch(mx4_dequantize_kernel<__bf16, true>, (__bf16*)x) : launch(mx4_dequantize_kernel<__bf16, false>, (__bf16*)x);
+    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (float*)x);
+    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_dequantize_kernel<_Float16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (_Float16*)x);
+    else hipLaunchKernelGGL(mx4_dequantize_kernel<__bf16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (__bf16*)x);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }
@@ -678,15 +652,10 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     a.M = u->M; a.K = u->K; a.N = u->N; a.S = (u->K + MX4_K - 1) / MX4_K;
     a.x = u->x; a.x_type = u->x_type; a.ldx = u->ldx;
     if (u->x_type == UITK_T_MX4) a.x_scales = (const char*)u->x + mx4_records(u->M, u->K) * MX4_CODES;
-    else a.x_vec = aligned16(u->x) && (u->ldx * type_size(u->x_type)) % 16 == 0;
     a.w = (const char*)u->w; a.w_scales = a.w + mx4_records(u->N, u->K) * MX4_CODES;
     a.bias = u->bias; a.act = u->act; a.residual = u->residual; a.ldr = u->ldr;
     a.out = u->out; a.ldo = u->ldo; a.out_type = u->out_type;
     if (u->out_type == UITK_T_MX4) { a.out_S = (u->N + MX4_K - 1) / MX4_K; a.out_scales = (char*)u->out + mx4_records(u->M, u->N) * MX4_CODES; }
-    else {
-        const int sz = type_size(u->out_type), grp = 4 * sz;
-        a.vec4 = (uintptr_t)u->out % grp == 0 && u->ldo % 4 == 0 && (!u->residual || ((uintptr_t)u->residual % grp == 0 && u->ldr % 4 == 0));
-    }
     hipStream_t s = (hipStream_t)stream;
     const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
     if (plan.quantize_first) {

@@ -73,22 +73,18 @@ def overlaps(a, b):
     return a0 < b1 and b0 < a1
 
 
-def check_vector(t, name, n, device):
-    """A per-channel parameter: [n] on `device` -> in float32, contiguous (None stays None)."""
+def check_vector(t, name, n, device, keep):
+    """A per-channel parameter: [n] on `device` -> the address of its values in float32 (0: None).  What had to be converted joins `keep`."""
     if t is None:
-        return None
-    check_tensor(t, name)
+        return 0
+    if check_tensor(t, name) == _lib.T_F32 and t.get_device() == device.index and t.dim() == 1 and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dtype is not torch.float32:
-        t = t.to(torch.float32)
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def ptr(t):
-    return 0 if t is None else t.data_ptr()
+    keep.append(t.to(torch.float32).contiguous())
+    return keep[-1].data_ptr()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -181,7 +177,8 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
     to_mx4 = out_dtype == "mx4"
     if not to_mx4 and out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16, bfloat16 or 'mx4', got {out_dtype}")
-    b = check_vector(bias, "bias", N, device)
+    keep = []
+    b = check_vector(bias, "bias", N, device, keep)
     res, ldr = None, 0
     if residual is not None:
         if to_mx4:
@@ -210,6 +207,7 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
     src, ldx = (x.data, 0) if packed else as_rows(x, K)
     need = _workspace_bytes(M, N, K, x_type)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    args = _LINEAR_ARGS.pack(src.data_ptr(), w.data.data_ptr(), ptr(b), ptr(res), dst.data_ptr(), ptr(ws), M, N, K, ldx, ldr, N, x_type, out_type, _ACTS[act], 0)
+    args = _LINEAR_ARGS.pack(src.data_ptr(), w.data.data_ptr(), b, 0 if res is None else res.data_ptr(), dst.data_ptr(), 0 if ws is None else ws.data_ptr(),
+                             M, N, K, ldx, ldr, N, x_type, out_type, _ACTS[act], 0)
     run(_lib.packed("uitk_mx4_linear"), device, args)
     return result

@@ -13,21 +13,19 @@ import struct
 import torch
 
 from . import _lib
-from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, overlaps, ptr, run
+from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, overlaps, run
 
 _ARGS = struct.Struct("10Q7q8if4x")                                          # uitk_block_norm_args
 _KINDS = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
 
 
-def _affine(norm, name, D, device):
-    """(gain, offset), each [D] or None -> (given, gain, offset)"""
-    if norm is None:
-        return False, None, None
+def _affine(norm, name, D, device, keep):
+    """(gain, offset), each [D] or None -> their addresses"""
     try:
         w, b = norm
     except (TypeError, ValueError):
         raise TypeError(f"{name} must be a pair (weight, bias), each [{D}] or None") from None
-    return True, check_vector(w, f"{name} weight", D, device), check_vector(b, f"{name} bias", D, device)
+    return check_vector(w, name, D, device, keep), check_vector(b, name, D, device, keep)
 
 
 def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind="layer", eps=1e-6, out_dtype=None, inplace=False):
@@ -58,23 +56,27 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
         if y.shape != shape or y.device != device:
             raise ValueError(f"y must have the residual's shape and device, got {tuple(y.shape)} on {y.device}")
         yv, ldy = as_rows(y, D)
-    has_post, post_w, post_b = _affine(post, "post", D, device)
-    has_pre, pre_w, pre_b = _affine(pre, "pre", D, device)
-    s = check_vector(scale, "scale", D, device)
-    g, ldg, gate_rows, gate_type = None, 0, 1, 0
+    keep = []
+    post_w, post_b = (0, 0) if post is None else _affine(post, "post", D, device, keep)
+    pre_w, pre_b = (0, 0) if pre is None else _affine(pre, "pre", D, device, keep)
+    s = 0 if scale is None else check_vector(scale, "scale", D, device, keep)
+    g, ldg, gate_rows, gate_type = 0, 0, 1, 0
     if gate is not None:
         gate_type = check_tensor(gate, "gate")
         if gate.device != device:
             raise ValueError(f"gate is on {gate.device}, not on {device}")
-        if gate.shape != shape:
-            if len(shape) < 3 or gate.shape not in ((shape[0], D), (shape[0],) + (1,) * (len(shape) - 2) + (D,)):
-                raise ValueError(f"gate must be {tuple(shape)} (per token) or {(shape[0], D)} for a y of three or more dimensions (per sequence), got {tuple(gate.shape)}")
+        gs = gate.shape
+        if gs != shape:
+            if len(shape) < 3 or not (gs[0] == shape[0] and gs[-1] == D and gate.numel() == gs[0] * D and len(gs) in (2, len(shape))):
+                raise ValueError(f"gate must be {tuple(shape)} (per token) or {(shape[0], D)} for a y of three or more dimensions (per sequence), got {tuple(gs)}")
             gate_rows = max(1, rows // max(1, shape[0]))
-        g, ldg = as_rows(gate, D)
+        gv, ldg = as_rows(gate, D)
+        keep.append(gv)
+        g = gv.data_ptr()
     if out_dtype is None:
         out_dtype = residual.dtype
     h, h_type, h_ptr = None, 0, 0
-    if has_pre:
+    if pre is not None:
         if out_dtype == "mx4":
             h, h_type = Mx4Tensor.empty(shape, device), _lib.T_MX4
             h_ptr = h.data.data_ptr()
@@ -87,7 +89,7 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
     if y is None:
         r_out, ro, ldro = residual, None, 0
     elif inplace:
-        for name, t in (("gate", gate), ("scale", scale), ("post weight", post_w), ("post bias", post_b), ("pre weight", pre_w), ("pre bias", pre_b)):
+        for name, t in (("gate", gate), ("scale", scale)) + tuple(("post", t) for t in post or ()) + tuple(("pre", t) for t in pre or ()):
             if t is not None and overlaps(residual, t):
                 raise ValueError(f"inplace: {name} shares memory with the residual")
         if overlaps(residual, y) and not (residual.data_ptr() == y.data_ptr() and residual.stride() == y.stride() and residual.dtype == y.dtype):
@@ -100,7 +102,7 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
         ldro = D
     if rows == 0:
         return r_out, h
-    args = _ARGS.pack(ptr(yv), r.data_ptr(), ptr(ro), h_ptr, ptr(g), ptr(s), ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b),
-                      rows, ldy, ldr, ldro, D, ldg, gate_rows, D, y_type, r_type, h_type, gate_type, _KINDS[kind], has_post, has_pre, eps)
+    args = _ARGS.pack(0 if yv is None else yv.data_ptr(), r.data_ptr(), 0 if ro is None else ro.data_ptr(), h_ptr, g, s, post_w, post_b, pre_w, pre_b,
+                      rows, ldy, ldr, ldro, D, ldg, gate_rows, D, y_type, r_type, h_type, gate_type, _KINDS[kind], post is not None, pre is not None, eps)
     run(_lib.packed("uitk_block_norm"), device, args)
     return r_out, h
