@@ -218,8 +218,8 @@ def test_linear_epilogue(M, N, K, act, out_dtype):
     check_linear(acc, x, w, None, act, res)
 
 
-# what the tile kernels take: more than 64 tiles of 128 x 128; at least 512 of 256 x 128 and K >= 2048 (ragged edges in every direction)
-TILES = [(1100, 1030, 130), (1024, 1280, 64), (3000, 520, 400), (16385, 513, 2049), (128 * 128, 1024, 2048)]
+# what the tile kernels take: more than 128 tiles of 128 x 128; at least 512 of 256 x 128 and K >= 4096 (ragged edges in every direction)
+TILES = [(1100, 1930, 130), (1024, 2304, 64), (3000, 920, 400), (16385, 513, 2049), (128 * 128, 1024, 2048), (8193, 2049, 4097), (8192, 2048, 4096)]
 
 
 @gpu
@@ -248,7 +248,7 @@ def test_linear_many_rows(M, N, K, packed, out_dtype):
 
 
 @gpu
-@pytest.mark.parametrize("M,N,K", [(1100, 1030, 130), (16385, 260, 2049), (700, 2000, 256)])
+@pytest.mark.parametrize("M,N,K", [(1100, 1930, 130), (16385, 1030, 4200), (700, 3000, 256)])
 def test_linear_many_rows_to_four_bits_and_into_a_view(M, N, K):
     x, w = mx4.quantize(_rand((M, K), torch.float16, seed=M).cuda()), mx4.quantize((_rand((N, K), torch.float32, seed=K) * K ** -0.5).cuda())
     f = mx4.linear(x, w, act="relu", out_dtype=torch.float32)

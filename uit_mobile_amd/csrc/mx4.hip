@@ -272,10 +272,12 @@ __global__ void __launch_bounds__(64 * NW) mx4_rows_kernel(Mx4LinearArgs a) {
 
 // ---- many rows: both operands packed, a workgroup computes BN outputs x BM tokens from LDS.
 // A stage holds 128 elements of K: BN / 64 + BM / 64 records, brought in by LDS-DMA in the order they have in memory (a record IS its
-// LDS image: every fragment read is 1 KB of consecutive bytes, no bank conflicts, no address arithmetic).  Three slots: while the waves
-// multiply stage s, stages s + 1 and s + 2 are on their way; the slot of s is free once its second half is in registers.
-// One barrier per stage, placed between the two halves: the fragments of the half in front of it are in registers already, so the
-// matrix pipe has work while the waves meet.
+// LDS image: every fragment read is 1 KB of consecutive bytes, no bank conflicts, no address arithmetic).  Two slots: stage s + 1 is on
+// its way while s is multiplied, s + 2 follows into the slot of s once the second half of s is in registers.  One barrier per stage,
+// between the two halves, and every load issued behind a product, so that the matrix pipe has work throughout.  (A third slot costs a
+// workgroup per CU and is slower: 16128 x 2304 x 768, 128 x 128 tile, 3 / 2 slots 32.5 / 28.7 us; 8192^3, 256 x 128: 265 / 262; loads behind products instead of in one go: 254.)
+// 8192^3: 4.3 PFLOP/s at 1.7 GHz and 53 % matrix-pipe occupancy: the card is at its power limit (products from registers alone, on the same
+// random operands: 6.3 PFLOP/s at 1.55 GHz; on zeros 9.7 at 2.4).  Narrow K: bound by writing the output (16128 x 2304 x 768: 81 MB, 2.9 TB/s).
 __device__ __forceinline__ void mx4_dma16(unsigned lds, unsigned off, const char* src) {       // 64 lanes x 16 B -> 1 KB at lds
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(src) : "memory", "m0");
 }
@@ -290,7 +292,7 @@ struct Mx4Tile {
     static constexpr int RN = BN / 64, RM = BM / 64, REC = RN + RM;         // records of a stage
     static constexpr int TN = BN / WN / 32, TM = BM / WM / 32;              // 32 x 32 tiles of a wave
     static constexpr int STAGE = REC * (MX4_CODES + MX4_SCALES);
-    static constexpr int SLOTS = 3;
+    static constexpr int SLOTS = 2;
     static constexpr int CP = REC * 4 / NW, SP = (REC + NW - 1) / NW;       // pieces of codes (1 KB) / of scales (256 B) a wave brings in per stage
     static constexpr int LOADS = CP + SP;
     static constexpr int LDE = TN * 32 + 4;                                 // floats per token row of the epilogue's buffer
@@ -394,13 +396,14 @@ __global__ void __launch_bounds__(64 * WN * WM, BN * BM <= 256 * 128 ? 2 : 1) mx
     for (int i = 0; i < T::SP; ++i) src_scales[i] = record(min(wave * T::SP + i, T::REC - 1), true);
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const unsigned off16 = lane * 16, off4 = lane * 4;
-    auto bring = [&](int s) {
+    // piece i of what this wave brings in for stage s: CP pieces of codes, then SP of scales
+    auto bring = [&](int s, int i) {
         const unsigned slot = lds0 + (s % T::SLOTS) * T::STAGE;
-#pragma unroll
-        for (int i = 0; i < T::CP; ++i) mx4_dma16(slot + (wave * T::CP + i) * 1024, off16, src_codes[i] + (int64_t)s * MX4_CODES);
-#pragma unroll
-        for (int i = 0; i < T::SP; ++i)
-            mx4_dma4(slot + T::REC * MX4_CODES + min(wave * T::SP + i, T::REC - 1) * MX4_SCALES, off4, src_scales[i] + (int64_t)s * MX4_SCALES);
+        if (i < T::CP) mx4_dma16(slot + (wave * T::CP + i) * 1024, off16, src_codes[i] + (int64_t)s * MX4_CODES);
+        else {
+            const int j = i - T::CP;
+            mx4_dma4(slot + T::REC * MX4_CODES + min(wave * T::SP + j, T::REC - 1) * MX4_SCALES, off4, src_scales[j] + (int64_t)s * MX4_SCALES);
+        }
     };
     const int wn = wave / WM, wm = wave % WM;                               // the wave's place in the tile
     // row tile j of the wave: rows 32 (wn TN + j) of the tile = record (..) / 2, half (..) % 2 of it.  TN and TM are even or the wave's
@@ -408,19 +411,16 @@ __global__ void __launch_bounds__(64 * WN * WM, BN * BM <= 256 * 128 ? 2 : 1) mx
     static_assert(T::TN % 2 == 0 && T::TM % 2 == 0, "a wave owns whole records");
     mx_i4 fa[2][T::TN], fb[2][T::TM];
     int sa[T::TN / 2], sb[T::TM / 2];
-    auto fetch = [&](int s, int kh, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM]) {
-        const char* slot = lds + (s % T::SLOTS) * T::STAGE;
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) A[j] = *(const mx_i4*)(slot + (wn * T::TN / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
-#pragma unroll
-        for (int j = 0; j < T::TM; ++j) B[j] = *(const mx_i4*)(slot + (T::RN + wm * T::TM / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
+    // fragment i of half kh of a stage: the first of each operand first, so that a product can start
+    constexpr int FRAGS = T::TN + T::TM, SCALES = (T::TN + T::TM) / 2;
+    auto fetch = [&](const char* slot, int kh, int i, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM]) {
+        const int j = i < 2 * T::TM ? i / 2 : i - T::TM;                    // (TM <= TN: A0 B0 A1 B1 .. then the rest of A)
+        if (i < 2 * T::TM && i % 2) B[j] = *(const mx_i4*)(slot + (T::RN + wm * T::TM / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
+        else A[j] = *(const mx_i4*)(slot + (wn * T::TN / 2 + j / 2) * MX4_CODES + (2 * (j & 1) + kh) * 1024 + lane * 16);
     };
-    auto fetch_scales = [&](int s, int (&A)[T::TN / 2], int (&B)[T::TM / 2]) {
-        const char* slot = lds + (s % T::SLOTS) * T::STAGE + T::REC * MX4_CODES;
-#pragma unroll
-        for (int j = 0; j < T::TN / 2; ++j) A[j] = *(const int*)(slot + (wn * T::TN / 2 + j) * MX4_SCALES + lane * 4);
-#pragma unroll
-        for (int j = 0; j < T::TM / 2; ++j) B[j] = *(const int*)(slot + (T::RN + wm * T::TM / 2 + j) * MX4_SCALES + lane * 4);
+    auto fetch_scale = [&](const char* slot, int i, int (&A)[T::TN / 2], int (&B)[T::TM / 2]) {
+        if (i < T::TN / 2) A[i] = *(const int*)(slot + T::REC * MX4_CODES + (wn * T::TN / 2 + i) * MX4_SCALES + lane * 4);
+        else B[i - T::TN / 2] = *(const int*)(slot + T::REC * MX4_CODES + (T::RN + wm * T::TM / 2 + i - T::TN / 2) * MX4_SCALES + lane * 4);
     };
     mx_f16 acc[T::TN][T::TM];
 #pragma unroll
@@ -429,52 +429,80 @@ __global__ void __launch_bounds__(64 * WN * WM, BN * BM <= 256 * 128 ? 2 : 1) mx
         for (int j = 0; j < T::TM; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    auto multiply = [&](auto KH, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM], int (&SA)[T::TN / 2], int (&SB)[T::TM / 2]) {
+    // one half of a stage; between(i) is what else is issued behind product i: the matrix pipe is busy for 32 cycles with each, and a wave
+    // that issues its loads in one go instead leaves it idle meanwhile
+    constexpr int PROD = T::TN * T::TM;
+    auto multiply = [&](auto KH, mx_i4 (&A)[T::TN], mx_i4 (&B)[T::TM], int (&SA)[T::TN / 2], int (&SB)[T::TM / 2], auto between) {
         constexpr int kh = decltype(KH)::value;
 #pragma unroll
         for (int i = 0; i < T::TN; i += 2)
 #pragma unroll
             for (int j = 0; j < T::TM; j += 2) {
+                const int p = (i / 2 * (T::TM / 2) + j / 2) * 4;
                 acc[i][j] = mx4_mfma<kh, kh>(A[i], B[j], acc[i][j], SA[i / 2], SB[j / 2]);
+                between(p);
                 acc[i + 1][j] = mx4_mfma<2 + kh, kh>(A[i + 1], B[j], acc[i + 1][j], SA[i / 2], SB[j / 2]);
+                between(p + 1);
                 acc[i][j + 1] = mx4_mfma<kh, 2 + kh>(A[i], B[j + 1], acc[i][j + 1], SA[i / 2], SB[j / 2]);
+                between(p + 2);
                 acc[i + 1][j + 1] = mx4_mfma<2 + kh, 2 + kh>(A[i + 1], B[j + 1], acc[i + 1][j + 1], SA[i / 2], SB[j / 2]);
+                between(p + 3);
             }
     };
     std::integral_constant<int, 0> K0;
     std::integral_constant<int, 1> K1;
     // ---- the pipeline
-    for (int s = 0; s < 3 && s < S; ++s) bring(s);
-    if (S >= 3) mx4_wait_dma<2 * T::LOADS>(); else if (S == 2) mx4_wait_dma<T::LOADS>(); else mx4_wait_dma<0>();
+    for (int s = 0; s < T::SLOTS && s < S; ++s) {
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) bring(s, i);
+    }
+    if (S > 1) mx4_wait_dma<T::LOADS>(); else mx4_wait_dma<0>();            // stage 0 is here
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    fetch(0, 0, fa[0], fb[0]);
-    fetch_scales(0, sa, sb);
-    for (int s = 0; s + 1 < S; ++s) {
-        fetch(s, 1, fa[1], fb[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(K0, fa[0], fb[0], sa, sb);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < FRAGS; ++i) fetch(lds, 0, i, fa[0], fb[0]);
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) fetch_scale(lds, i, sa, sb);
+    constexpr int PER_F = (FRAGS + PROD - 1) / PROD, PER_S = (SCALES + PROD - 1) / PROD, PER_L = (T::LOADS + PROD - 1) / PROD;
+    auto step = [&](int s, auto MORE) {                                     // MORE: stage s + 2 exists
+        const char* slot = lds + s % T::SLOTS * T::STAGE;
+        const char* next = lds + (s + 1) % T::SLOTS * T::STAGE;
+        multiply(K0, fa[0], fb[0], sa, sb, [&](int p) {
+#pragma unroll
+            for (int i = p * PER_F; i < (p + 1) * PER_F; ++i) if (i < FRAGS) fetch(slot, 1, i, fa[1], fb[1]);
+            __builtin_amdgcn_sched_barrier(0);
+        });
         // stage s + 1 has landed (this wave's part; the barrier says so for all), and this wave is done reading the slot of s
-        if (s + 2 < S) mx4_wait_dma<T::LOADS>(); else mx4_wait_dma<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 3 < S) bring(s + 3);
         int oa[T::TN / 2], ob[T::TM / 2];                                   // the scales of the half that is still to be multiplied
 #pragma unroll
         for (int i = 0; i < T::TN / 2; ++i) oa[i] = sa[i];
 #pragma unroll
         for (int i = 0; i < T::TM / 2; ++i) ob[i] = sb[i];
-        fetch(s + 1, 0, fa[0], fb[0]);
-        fetch_scales(s + 1, sa, sb);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(K1, fa[1], fb[1], oa, ob);
-        __builtin_amdgcn_sched_barrier(0);
+        multiply(K1, fa[1], fb[1], oa, ob, [&](int p) {
+#pragma unroll
+            for (int i = p * PER_F; i < (p + 1) * PER_F; ++i) if (i < FRAGS) fetch(next, 0, i, fa[0], fb[0]);
+#pragma unroll
+            for (int i = p * PER_S; i < (p + 1) * PER_S; ++i) if (i < SCALES) fetch_scale(next, i, sa, sb);
+            if constexpr (decltype(MORE)::value) {
+#pragma unroll
+                for (int i = p * PER_L; i < (p + 1) * PER_L; ++i) if (i < T::LOADS) bring(s + T::SLOTS, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    {
+        int s = 0;
+        for (; s + T::SLOTS < S; ++s) step(s, std::true_type{});
+        for (; s + 1 < S; ++s) step(s, std::false_type{});
+        const char* slot = lds + (S - 1) % T::SLOTS * T::STAGE;
+#pragma unroll
+        for (int i = 0; i < FRAGS; ++i) fetch(slot, 1, i, fa[1], fb[1]);
+        multiply(K0, fa[0], fb[0], sa, sb, [](int) {});
+        multiply(K1, fa[1], fb[1], sa, sb, [](int) {});
     }
-    fetch(S - 1, 1, fa[1], fb[1]);
-    multiply(K0, fa[0], fb[0], sa, sb);
-    multiply(K1, fa[1], fb[1], sa, sb);
     __syncthreads();                                                        // every wave has left the ring
     // ---- epilogue: 32 tokens at a time through the wave's own part of LDS, so that a lane holds four consecutive outputs of a token and
     // a wave stores whole rows (straight from the accumulators a row would leave in pieces of 16 bytes)
@@ -541,24 +569,24 @@ static hipError_t mx4_launch_rows(Mx4LinearArgs& a, hipStream_t s) {
     return go(mx4_rows_kernel<NT, NW, __bf16, false>);
 }
 
-// Which kernel, and whether activations that are not packed are quantised inside it.  us on the GPU, launches back to back in a graph:
-// * rows against tiles: 128 x 128 tiles need more than 128 of them (packed x; rows / 128 x 128 / 256 x 128: 256 x 8192 x 8192: 20 / 26 / 41;
-//   512 x 4096 x 4096: 15 / 16 / 24; 2048 x 2048 x 2048: 17 / 12 / 17), the wide ones two workgroups on every CU and a K that outweighs
-//   their longer epilogue (16128 x 2304 x 768: - / 33 / 38; 4096 x 4096 x 4096: 95 / 47 / 42; 8192 x 8192 x 8192: 658 / 304 / 281).
+// Which kernel, and whether activations that are not packed are quantised inside it.  us on the GPU, packed x unless said otherwise:
+// * rows against tiles: 128 x 128 tiles need more than 128 of them (rows / 128 x 128: 512 x 4096 x 4096: 12.5 / 13.1; 128 x 16384 x 4096: 15.7 / 19.2;
+//   300 x 8192 x 512: 7.7 / 6.1; 2048 x 4096 x 2048: 31 / 16), 256 x 128 ones two workgroups on every CU and a K that outweighs their longer
+//   epilogue (128 x 128 / 256 x 128: 16128 x 2304 x 768: 28.7 / 36.8; 16128 x 2304 x 2048: 50.4 / 55.2; 4096 x 4096 x 4096: 41.3 / 40.1; 8192 x 8192 x 8192: 270 / 254).
 // * rows: 8 waves share K, 16 where a wave would still have two records or more (13 x 8192 x 8192, 8 / 16: 12.5 / 11.9); with more than 512
 //   workgroups 64 columns each instead of 32 (128 x 8192 x 8192, 32 / 64: 21.4 / 17.5).
-// * quantising inside repeats the work in every column group, about 65 vector instructions per 32 x 64 fragment, and costs more than a
-//   launch of its own (2.6 us) from 4096 fragments on: inside / packed: 1 x 2304 x 768 (864 fragments) 4.4 / 3.2, 252 x 768 x 768 (2304) 4.9 / 3.4,
-//   252 x 2304 x 768 (6912) 7.4 / 4.1, 13 x 8192 x 8192 (32768) 17.7 / 11.9.
+// * quantising inside repeats the work in every column group, about 65 vector instructions per 32 x 64 fragment; a launch of its own costs
+//   2.6 us of the GPU, and a caller that does not replay a graph 3 us of the host and a workspace.  bf16 inside / packed, GPU: 1 x 2304 x 768 (864
+//   fragments) 4.4 / 3.2, 252 x 768 x 768 (2304) 4.9 / 3.4, 1003 x 537 x 1000 (8704) 11 / 5.1, 64 x 4096 x 4096 (16384) 12.4 / 6.0, 13 x 8192 x 8192 (32768) 17.7 / 11.9.
 enum { MX4_ROWS8 = 0, MX4_ROWS16, MX4_ROWS64, MX4_TILE128, MX4_TILE256 };
 struct Mx4Plan { int kernel; bool quantize_first; };
 static Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t K, int x_type) {
     const int64_t m128 = (M + 127) / 128, S = (K + MX4_K - 1) / MX4_K, groups = ((N + 31) / 32) * ((M + 31) / 32);
     Mx4Plan p{MX4_ROWS8, x_type != MT_MX4};
-    if (M > 64 && m128 * ((N + 127) / 128) > 128) p.kernel = m128 * ((N + 255) / 256) >= 512 && K >= 2048 ? MX4_TILE256 : MX4_TILE128;
+    if (M > 64 && m128 * ((N + 127) / 128) > 128) p.kernel = m128 * ((N + 255) / 256) >= 512 && K >= 4096 ? MX4_TILE256 : MX4_TILE128;
     else if (groups > 512) p.kernel = MX4_ROWS64;
     else if (S >= 32) p.kernel = MX4_ROWS16;
-    if (p.kernel < MX4_TILE128 && 2 * groups * S <= 4096) p.quantize_first = false;
+    if (p.kernel < MX4_TILE128 && 2 * groups * S <= 10240) p.quantize_first = false;
     return p;
 }
 
@@ -657,7 +685,12 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     a.out = u->out; a.ldo = u->ldo; a.out_type = u->out_type;
     if (u->out_type == UITK_T_MX4) { a.out_S = (u->N + MX4_K - 1) / MX4_K; a.out_scales = (char*)u->out + mx4_records(u->M, u->N) * MX4_CODES; }
     hipStream_t s = (hipStream_t)stream;
+#ifdef UITK_LAB
+    Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
+    if (u->reserved) { plan.kernel = u->reserved - 1; plan.quantize_first = u->x_type != UITK_T_MX4 && plan.kernel >= MX4_TILE128; }
+#else
     const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
+#endif
     if (plan.quantize_first) {
         if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
         if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;

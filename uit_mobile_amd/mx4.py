@@ -62,15 +62,22 @@ def as_rows(t, K):
     return v, (v.stride(0) if rows > 1 else K)
 
 
+def span(t):
+    """The addresses a tensor's elements lie between (rows of one buffer that interleave count as sharing it)."""
+    lo = t.data_ptr()
+    if t.is_contiguous() or not t.numel():
+        return lo, lo + t.numel() * t.element_size()
+    return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def overlaps(a, b):
-    """Do two CUDA tensors share memory?  (By the spans their strides reach over: rows of one buffer that interleave count as sharing.)"""
-    def span(t):
-        lo = t.data_ptr()
-        return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
-    if a.device != b.device or not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    """Do two spans share memory?"""
+    return a[0] < b[1] and b[0] < a[1]
+
+
+def new(shape, dtype, like):
+    """An empty tensor on like's device (new_empty costs half of torch.empty where the type is the same)."""
+    return like.new_empty(shape) if like.dtype is dtype else torch.empty(shape, dtype=dtype, device=like.device)
 
 
 def check_vector(t, name, n, device, keep):
@@ -191,16 +198,17 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
             raise ValueError("out is not supported for a 4-bit output")
         if out.shape != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {tuple(shape)} {out_dtype} on {device}")
+        mine = span(out)
         for name, t in (("x", x.data if packed else x), ("w", w.data), ("bias", bias)):
-            if t is not None and overlaps(out, t):
+            if t is not None and overlaps(mine, span(t)):
                 raise ValueError(f"out shares memory with {name}")
-        if residual is not None and overlaps(out, residual) and not (out.data_ptr() == residual.data_ptr() and residual.is_contiguous()):
+        if residual is not None and overlaps(mine, span(residual)) and not (out.data_ptr() == residual.data_ptr() and residual.is_contiguous()):
             raise ValueError("out shares memory with the residual without being the residual")
     if to_mx4:
         result = Mx4Tensor.empty(shape, device)
         dst, out_type = result.data, _lib.T_MX4
     else:
-        result = dst = torch.empty(shape, dtype=out_dtype, device=device) if out is None else out
+        result = dst = new(shape, out_dtype, w.data if packed else x) if out is None else out
         out_type = _TYPES[out_dtype]
     if M == 0:
         return result

@@ -13,7 +13,7 @@ import struct
 import torch
 
 from . import _lib
-from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, overlaps, run
+from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, new, overlaps, run, span
 
 _ARGS = struct.Struct("10Q7q8if4x")                                          # uitk_block_norm_args
 _KINDS = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
@@ -81,7 +81,7 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
             h, h_type = Mx4Tensor.empty(shape, device), _lib.T_MX4
             h_ptr = h.data.data_ptr()
         elif out_dtype in _TYPES:
-            h, h_type = torch.empty(shape, dtype=out_dtype, device=device), _TYPES[out_dtype]
+            h, h_type = new(shape, out_dtype, residual), _TYPES[out_dtype]
             h_ptr = h.data_ptr()
         else:
             raise TypeError(f"out_dtype must be float32, float16, bfloat16 or 'mx4', got {out_dtype}")
@@ -89,16 +89,17 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
     if y is None:
         r_out, ro, ldro = residual, None, 0
     elif inplace:
+        mine = span(residual)
         for name, t in (("gate", gate), ("scale", scale)) + tuple(("post", t) for t in post or ()) + tuple(("pre", t) for t in pre or ()):
-            if t is not None and overlaps(residual, t):
+            if t is not None and overlaps(mine, span(t)):
                 raise ValueError(f"inplace: {name} shares memory with the residual")
-        if overlaps(residual, y) and not (residual.data_ptr() == y.data_ptr() and residual.stride() == y.stride() and residual.dtype == y.dtype):
+        if overlaps(mine, span(y)) and not (residual.data_ptr() == y.data_ptr() and residual.stride() == y.stride() and residual.dtype == y.dtype):
             raise ValueError("inplace: y shares memory with the residual without being the residual")
         if rows and r.data_ptr() != residual.data_ptr():
             raise ValueError("inplace: the residual's rows cannot be addressed in place (its strides need a copy)")
         r_out, ro, ldro = residual, r, ldr
     else:
-        r_out = ro = torch.empty(shape, dtype=residual.dtype, device=device)
+        r_out = ro = residual.new_empty(shape)
         ldro = D
     if rows == 0:
         return r_out, h
