@@ -396,7 +396,7 @@ typedef struct uitk_block_norm_args {
     const void* y;                         /* [rows, D] the block's output, or NULL */
     const void* residual;                  /* [rows, D] */
     void* residual_out;                    /* [rows, D] of r_type; may be `residual` itself */
-    void* h;                               /* [rows, D] of h_type, or packed (UITK_T_MX4) */
+    void* h;                               /* [rows, D] of h_type, or packed (UITK_T_MX4); may be `y` itself where type and rows agree */
     const void* gate;                      /* row m of the stream uses gate row m / gate_rows: 1 = per token, T = per sequence; or NULL */
     const float* scale;                    /* [D] or NULL */
     const float *post_w, *post_b;          /* [D]; NULL: no gain / no offset */

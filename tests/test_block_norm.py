@@ -86,7 +86,7 @@ def test_refusals_before_any_launch():
     for kw in (dict(rows=-1), dict(D=0), dict(D=16385), dict(r_type=3), dict(y_type=3), dict(h_type=4), dict(kind=2), dict(eps=-1.0), dict(eps=float("nan")),
                dict(y=None, post=1), dict(y=None, pre=0), dict(residual=None), dict(residual_out=None), dict(h=None), dict(ldy=31), dict(ldr=31), dict(ldro=31),
                dict(ldh=31), dict(gate=1 << 23, ldg=31), dict(gate=1 << 23, ldg=32, gate_rows=0), dict(gate=1 << 23, ldg=32, gate_type=3),
-               dict(h_type=3, h=(1 << 22) + 8)):
+               dict(h_type=3, h=(1 << 22) + 8), dict(y=(1 << 20) + 2), dict(scale=(1 << 24) + 2), dict(h=(1 << 22) + 1, h_type=1), dict(pre_w=(1 << 24) + 1)):
         assert call(**kw) == _lib.ERR_INVALID_ARG, kw
     assert call(rows=0, residual=None) == 0
     assert L.uitk_block_norm(None, None) == _lib.ERR_INVALID_ARG
@@ -233,3 +233,27 @@ def test_refusals():
         norms.block_norm(flat[1:385].view(2, 3, 64), flat[:384].view(2, 3, 64), inplace=True)
     with pytest.raises(RuntimeError, match="gradient"):
         norms.block_norm(y.clone().requires_grad_(), y)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    D = 4096
+    rows = (1 << 31) // D + 77
+    y, r = torch.zeros((rows, D), dtype=torch.bfloat16, device="cuda"), torch.zeros((rows, D), dtype=torch.bfloat16, device="cuda")
+    ty, tr, _, pre, _, _ = _make((50, D), torch.bfloat16, torch.bfloat16, seed=4)
+    y[-50:], r[-50:] = ty.cuda(), tr.cuda()
+    got = norms.block_norm(y, r, pre=_dev(pre))
+    want = norms.block_norm(ty.cuda(), tr.cuda(), pre=_dev(pre))
+    assert torch.equal(got[0][-50:], want[0]) and torch.equal(got[1][-50:], want[1])
+
+
+@gpu
+def test_parameters_and_gates_of_other_types_and_strides():
+    y, r, post, pre, gate, scale = _make((3, 4, 130), torch.float32, torch.float32, seed=9, gate="row")
+    h16 = lambda t: None if t is None else t.half()
+    po, pr, sc = tuple(map(h16, post)), tuple(map(h16, pre)), h16(scale)
+    got = norms.block_norm(*_dev((y, r)), post=_dev(po), pre=_dev(pr), scale=torch.stack([sc, sc], 1).cuda()[:, 0], gate=gate.bfloat16().t().contiguous().cuda().t())
+    check(got, y, r, tuple(t.float() for t in po), gate.bfloat16().float(), sc.float(), tuple(t.float() for t in pr))
+    tok = torch.rand(3, 4, 1).expand(3, 4, 130)
+    got = norms.block_norm(*_dev((y, r)), gate=tok.cuda().expand(3, 4, 130))
+    check(got, y, r, gate=tok)

@@ -78,6 +78,14 @@ def test_refusals_before_any_launch():
                dict(w=(1 << 21) + 4), dict(residual=1 << 23, ldr=7), dict(residual=1 << 23, ldr=8, out_type=3), dict(x_type=3, x=(1 << 20) + 8),
                dict(out_type=3, out=(1 << 22) + 8)):
         assert call(**kw) == bad, kw
+    for kw in (dict(x=(1 << 20) + 2), dict(out=(1 << 22) + 1, out_type=1), dict(bias=(1 << 23) + 2), dict(residual=(1 << 23) + 1, ldr=8, out_type=2)):
+        assert call(**kw) == bad, kw
+    big = dict(M=4096, N=4096, K=4096, ldx=4096, ldo=4096)                   # packs x first: needs the workspace it asked for
+    assert L.uitk_mx4_linear_workspace(4096, 4096, 4096, 0) == L.uitk_mx4_bytes(4096, 4096) and L.uitk_mx4_linear_workspace(4096, 4096, 4096, 3) == 0
+    assert call(**big) == bad and call(workspace=(1 << 24) + 8, **big) == bad
+    assert L.uitk_mx4_linear_workspace(1, 64, 64, 0) == 0
+    assert L.uitk_mx4_quantize(ctypes.c_void_p((1 << 20) + 1), 1, 4, 32, 32, p, None) == bad
+    assert L.uitk_mx4_dequantize(p, 4, 32, ctypes.c_void_p((1 << 20) + 2), 0, 32, None) == bad
     assert call(M=0, x=None) == 0
     assert L.uitk_mx4_linear_workspace(4, 8, 32, 5) == -1 and L.uitk_mx4_linear_workspace(4, 0, 32, 0) == -1
 
@@ -384,3 +392,84 @@ def test_refusals():
         mx4.quantize(p)
     with torch.no_grad():
         mx4.quantize(p)
+
+
+@gpu
+def test_packed_matrices_are_checked_where_they_are_made():
+    q = mx4.quantize(_rand((70, 200), torch.float32).cuda())
+    again = mx4.Mx4Tensor(q.data, (70, 200))
+    assert torch.equal(again.dequantize(), q.dequantize()) and "70" in repr(again)
+    assert torch.equal(mx4.Mx4Tensor(q.data, (7, 10, 200)).dequantize().view(70, 200), q.dequantize())
+    for data, shape in ((q.data, (129, 200)), (q.data, (70, 257)), (q.data[1:], (70, 200)), (q.data.cpu(), (70, 200)), (q.data.float(), (70, 200)), (q.data, ()), (None, (70, 200))):
+        with pytest.raises(ValueError):
+            mx4.Mx4Tensor(data, shape)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows of a large call are those of a small one."""
+    K = 4096
+    rows = (1 << 31) // K + 129
+    x = torch.empty((rows, K), dtype=torch.bfloat16, device="cuda")
+    x[:128] = 1.0
+    tail = _rand((200, K), torch.bfloat16, seed=1).cuda()
+    x[-200:] = tail
+    q = mx4.quantize(x)
+    assert torch.equal(q.dequantize(torch.bfloat16)[-200:], mx4.quantize(tail).dequantize(torch.bfloat16))
+    w = mx4.quantize((_rand((40, K), torch.float32, seed=2) * K ** -0.5).cuda())
+    got, want = mx4.linear(q, w)[-200:], mx4.linear(tail, w, out_dtype=torch.float32)
+    S = mx4.quantize(tail).dequantize().double().abs() @ w.dequantize().double().abs().T
+    assert ((got - want).abs().double() <= 2 * (2 * K / 64 + 16) * 2.0 ** -23 * S).all()
+    del x, q, got
+    M, N = 70000, 32768                                                      # an output of more than 2^31 elements
+    x, w = _rand((M, 64), torch.bfloat16, seed=3).cuda(), mx4.quantize(_rand((N, 64), torch.float32, seed=4).cuda())
+    y = mx4.linear(x, w)
+    a, b = mx4.quantize(x[-100:]).dequantize().double(), w.dequantize().double()
+    ref = a @ b.T
+    assert ((y[-100:].double() - ref).abs() <= 18 * 2.0 ** -23 * (a.abs() @ b.abs().T) + ref.abs() * 2.0 ** -8 + 1e-38).all()
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(13, 300, 8192), (1500, 2000, 512), (8192, 2048, 4096)])
+def test_every_kernel_under_capture_and_on_two_streams_at_once(M, N, K):
+    xs = [_rand((M, K), torch.bfloat16, seed=i).cuda() for i in range(2)]
+    w = mx4.quantize((_rand((N, K), torch.float32, seed=9) * K ** -0.5).cuda())
+    want = [mx4.linear(x, w, act="gelu") for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = mx4.linear(xs[i], w, act="gelu")
+    for i, s in enumerate(streams):
+        torch.cuda.current_stream().wait_stream(s)
+        got[i].record_stream(torch.cuda.current_stream())
+        assert torch.equal(got[i], want[i])
+    buf = xs[0].clone()
+    graphs = []
+    for _ in range(2):                                                       # two graphs of the same call, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = mx4.linear(buf, w, act="gelu")
+        graphs.append((g, out))
+    for i in (0, 1, 0, 1):
+        buf.copy_(xs[i])
+        for g, out in graphs:
+            g.replay()
+        assert torch.equal(mx4.linear(xs[1 - i], w, act="gelu"), want[1 - i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[i]) for _, out in graphs)
+
+
+@gpu
+def test_a_tensor_on_another_device_than_the_current_one_switches(monkeypatch):
+    """One device here: the current one is made to look like another, so the call takes the switching path."""
+    x, w = _rand((5, 64), torch.float32).cuda(), mx4.quantize(_rand((8, 64), torch.float32, seed=1).cuda())
+    want = mx4.linear(x, w)
+    seen = []
+    real = torch.cuda.device
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", lambda i: (seen.append(i), real(i))[1])
+    assert torch.equal(mx4.linear(x, w), want) and seen == [0]

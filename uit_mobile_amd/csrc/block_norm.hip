@@ -270,6 +270,10 @@ extern "C" int uitk_block_norm(const uitk_block_norm_args* u, void* stream) {
     if ((u->y && u->ldy < u->D) || u->ldr < u->D || (u->y && u->ldro < u->D) || (u->gate && u->ldg < u->D) || (u->pre && u->h_type != UITK_T_MX4 && u->ldh < u->D))
         return bad("rows overlap (a leading dimension below D)");
     if (u->pre && u->h_type == UITK_T_MX4 && ((uintptr_t)u->h & 15)) return bad("a packed h must be 16-byte aligned");
+    auto off = [](const void* p, int t) { return (uintptr_t)p % (t == UITK_T_F32 ? 4 : 2) != 0; };
+    if (off(u->residual, u->r_type) || (u->y && (off(u->y, u->y_type) || off(u->residual_out, u->r_type))) || (u->gate && off(u->gate, u->gate_type)) ||
+        (u->pre && u->h_type != UITK_T_MX4 && off(u->h, u->h_type)) || off(u->scale, 0) || off(u->post_w, 0) || off(u->post_b, 0) || off(u->pre_w, 0) || off(u->pre_b, 0))
+        return bad("a pointer is not aligned to its elements");
     BlockNormArgs a{};
     a.y = u->y; a.y_type = u->y_type; a.ldy = u->ldy; a.r = u->residual; a.r_type = u->r_type; a.ldr = u->ldr; a.rows = u->rows; a.D = u->D;
     a.rms = u->kind == UITK_NORM_RMS; a.eps = u->eps; a.post = u->post != 0; a.post_w = u->post_w; a.post_b = u->post_b;

@@ -19,74 +19,96 @@ namespace uitk {
 int set_error(int code, const std::string& msg);                          // api.cpp: the thread's uitk_last_error text
 
 // ------------------------------------------------------------------------------------------------------------------- quantize
-// One wave per record: lane (r = l % 32, g = l / 32) owns the blocks (row 32 rt + r, elements 64 kh + 32 g ..) of the four fragments,
-// so the maximum, the scale and the 16 bytes of a block never leave the lane, and a wave writes whole contiguous fragments.
-template <typename T>
+// One wave per record; 16 lanes share a row, a lane rounds 8 of its elements and four neighbours a block: a wave reads 128 consecutive elements
+// of four rows at a time, whatever their alignment, and finds a block's maximum in two lane exchanges.  (A whole block per lane needs no
+// exchange, but its 16-byte reads lie 64 or 128 bytes apart: 32768 x 4096 bf16 75 / 72 us (4.7 TB/s), 16384 x 4096 fp32 82 / 58, 32768 x 4095 bf16 137 / 102.)
+// SPLIT: the four waves of a workgroup share a record, 16 rows each: few records are a matter of latency.
+template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t K, int64_t ld, int64_t R, int64_t S,
                                                            char* __restrict__ codes, char* __restrict__ scales) {
-    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-    const int64_t rec = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ unsigned char sc[SPLIT ? 1 : 4][MX4_SCALES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, kb = l16 >> 2;       // the lane's block: half kb / 2, group kb % 2
+    const int64_t rec = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (rec >= R * S) return;
-    const int64_t rg = rec / S, s = rec - rg * S;
-    unsigned sc = 0;
+    const int64_t rg = rec / S, s = rec - rg * S, k = s * MX4_K + l16 * 8;
+    const int n = (int)min((int64_t)8, K - k);                              // (negative: no element of the row)
+    const int nrow = (int)min((int64_t)MX4_ROWS, rows - rg * MX4_ROWS);
+    const T* p = x + (rg * MX4_ROWS + (lane >> 4)) * ld + k;
+    char* c = codes + rec * MX4_CODES + (kb >> 1) * 1024 + ((kb & 1) * 32 + (lane >> 4)) * 16 + (l16 & 3) * 4;
+    unsigned char* my = sc[SPLIT ? 0 : wave];
+    constexpr int BATCH = sizeof(T) == 4 || SPLIT ? 4 : 8;                  // reads on their way at a time
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        const int64_t row = rg * MX4_ROWS + 32 * (f >> 1) + r, k = s * MX4_K + 64 * (f & 1) + 32 * g;
-        Mx4Block b{mx_i4{0, 0, 0, 0}, 0};
-        if (row < rows && k < K) {
-            Mx4Src<T> src;
-            src.load(x + row * ld + k, (int)min((int64_t)32, K - k));
-            b = src.pack();
+    for (int b0 = 0; b0 < (SPLIT ? 4 : 16); b0 += BATCH) {
+        const int i0 = SPLIT ? 4 * wave : b0;
+        if (4 * i0 >= nrow) break;                                          // (rows behind the matrix are left as they are)
+        Mx4Oct<T> v[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) v[i].load(p + (i0 + i) * 4 * ld, (i0 + i) * 4 + (lane >> 4) < nrow ? n : 0);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = (i0 + i) * 4;                                     // + lane / 16: the row of the record
+            const unsigned b = mx4_scale_byte(v[i].exponent());
+            const unsigned w = v[i].pack(mx4_scale_float(b));
+            *(unsigned*)(c + (r >> 5) * 2048 + (r & 31) * 16) = b == 255u ? 0u : w;
+            if ((l16 & 3) == 0) my[((kb & 1) * 32 + (r & 31) + (lane >> 4)) * 4 + 2 * (r >> 5) + (kb >> 1)] = (unsigned char)b;
         }
-        *(mx_i4*)(codes + rec * MX4_CODES + f * 1024 + lane * 16) = b.codes;
-        sc |= b.scale << (8 * f);
     }
-    *(unsigned*)(scales + rec * MX4_SCALES + lane * 4) = sc;
+    if constexpr (SPLIT) {
+        __syncthreads();
+        if (wave) return;
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");              // (LDS serves a wave in order: what is left to do is to keep the compiler's)
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    *(unsigned*)(scales + rec * MX4_SCALES + lane * 4) = *(const unsigned*)&my[lane * 4];
 }
 
-// One wave per record here too, but 16 lanes share a row: each turns four bytes of codes into eight elements, so that a wave stores 128
-// consecutive elements of four rows at a time (a whole block per lane would store 16-byte pieces 64 bytes apart).
+// One wave per record here too; a lane turns the codes of 16 bytes of output into them, so that neighbouring lanes store neighbouring
+// bytes of a row (a whole block per lane would store 16-byte pieces 64 or 128 bytes apart: 32768 x 4096 bf16 750 / 73 us, 4.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales, int64_t rows, int64_t K, int64_t ld,
                                                              int64_t R, int64_t S, T* __restrict__ x) {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, kb = l16 >> 2;      // the lane's block of its row: half kb / 2, group kb % 2
+    constexpr int P = 16 / sizeof(T), LPR = MX4_K / P, RPI = 64 / LPR;      // elements of a lane, lanes of a row, rows at a time
+    typedef T TP __attribute__((ext_vector_type(P)));
+    typedef T TPu __attribute__((ext_vector_type(P), aligned(sizeof(T))));
+    const int lane = threadIdx.x & 63, lr = lane % LPR, row0 = lane / LPR, kb = lr * P >> 5;          // the lane's block: half kb / 2, group kb % 2
     const int64_t rec = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (rec >= R * S) return;
-    const int64_t rg = rec / S, s = rec - rg * S, k = s * MX4_K + l16 * 8;
-    const int n = (int)min((int64_t)8, K - k);
-    const char* c = codes + rec * MX4_CODES + (kb >> 1) * 1024 + (kb & 1) * 512 + (l16 & 3) * 4;
+    const int64_t rg = rec / S, s = rec - rg * S, k = s * MX4_K + lr * P;
+    const int n = (int)min((int64_t)P, K - k), nrow = (int)min((int64_t)MX4_ROWS, rows - rg * MX4_ROWS);
+    const char* c = codes + rec * MX4_CODES + (kb >> 1) * 1024 + (kb & 1) * 512 + ((lr * P & 31) >> 1);
     const unsigned char* sc = (const unsigned char*)scales + rec * MX4_SCALES + (kb & 1) * 128 + (kb >> 1);
-#pragma unroll 4
-    for (int it = 0; it < 16; ++it) {
-        const int r = it * 4 + (lane >> 4);                                 // 0 .. 63
-        const int64_t row = rg * MX4_ROWS + r;
-        const unsigned w = *(const unsigned*)(c + (r >> 5) * 2048 + (r & 31) * 16);
-        const unsigned b = sc[(r & 31) * 4 + 2 * (r >> 5)];
-        const float f = mx4_scale_float(b);
-        float v[8];
-        const mx_f2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 1);
-        const mx_f2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 3);
-        v[0] = v0[0]; v[1] = v0[1]; v[2] = v1[0]; v[3] = v1[1]; v[4] = v2[0]; v[5] = v2[1]; v[6] = v3[0]; v[7] = v3[1];
-        if (b == 255u) {
+    if (n <= 0) return;
+    constexpr int BATCH = 8;                                                // rows asked for at a time
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
+    for (int i0 = 0; i0 < MX4_ROWS / RPI; i0 += BATCH) {
+        if (i0 * RPI >= nrow) return;
+        unsigned w[BATCH], b[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = (i0 + i) * RPI + row0;
+            const char* q = c + (r >> 5) * 2048 + (r & 31) * 16;
+            w[i] = P == 8 ? *(const unsigned*)q : *(const unsigned short*)q;
+            b[i] = sc[(r & 31) * 4 + 2 * (r >> 5)];
         }
-        if (row >= rows || n <= 0) continue;
-        T* o = x + row * ld + k;
-        if (n == 8) {
-            typedef T T8 __attribute__((ext_vector_type(16 / sizeof(T))));
-            typedef T T8u __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-            constexpr int P = 16 / sizeof(T);                               // elements of a 16-byte store
 #pragma unroll
-            for (int h = 0; h < 8 / P; ++h) {
-                T8 t;
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = (i0 + i) * RPI + row0;
+            const float f = mx4_scale_float(b[i]);
+            const mx_f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], f, 1),
+                                __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], f, 3)};
+            TP t;
 #pragma unroll
-                for (int i = 0; i < P; ++i) t[i] = (T)v[h * P + i];
-                *(T8u*)(o + h * P) = t;
+            for (int j = 0; j < P; ++j) t[j] = (T)(b[i] == 255u ? __uint_as_float(0x7fc00000u) : v[j >> 1][j & 1]);
+            if (r >= nrow) continue;
+            T* o = x + (rg * MX4_ROWS + r) * ld + k;
+            if (n == P) {
+                *(TPu*)o = t;
+            } else {
+#pragma unroll
+                for (int j = 0; j < P - 1; ++j) if (j < n) o[j] = t[j];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) if (i < n) o[i] = (T)v[i];
         }
     }
 }
@@ -548,6 +570,7 @@ static int mx4_check_matrix(const char* what, int64_t rows, int64_t K) {
     return UITK_OK;
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static bool on_element(const void* p, int type) { return (uintptr_t)p % (type == UITK_T_F32 ? 4 : 2) == 0; }
 
 template <int NT, int NW>
 static hipError_t mx4_launch_rows(Mx4LinearArgs& a, hipStream_t s) {
@@ -622,16 +645,19 @@ int uitk_mx4_quantize(const void* x, int type, int64_t rows, int64_t K, int64_t 
     if (rows == 0) return UITK_OK;
     if (!x || !q) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_quantize: null pointer");
     if (ld < K) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_quantize: rows overlap (ld < K)");
+    if (!on_element(x, type)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_quantize: x is not aligned to its elements");
     if (!aligned16(q)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_quantize: the packed buffer must be 16-byte aligned");
     const int64_t R = (rows + MX4_ROWS - 1) / MX4_ROWS, S = (K + MX4_K - 1) / MX4_K;
     char* codes = (char*)q;
     char* scales = codes + R * S * MX4_CODES;
     if ((R * S + 3) / 4 > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_quantize: more elements than one launch takes");
-    const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
+    const bool split = R * S <= 1024;                                       // (1021 x 1000 f16, a record to a workgroup / to a wave: 3.5 / 6.8 us)
+    const dim3 grid((unsigned)(split ? R * S : (R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_quantize_kernel<float>, grid, block, 0, s, (const float*)x, rows, K, ld, R, S, codes, scales);
-    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_quantize_kernel<_Float16>, grid, block, 0, s, (const _Float16*)x, rows, K, ld, R, S, codes, scales);
-    else hipLaunchKernelGGL(mx4_quantize_kernel<__bf16>, grid, block, 0, s, (const __bf16*)x, rows, K, ld, R, S, codes, scales);
+    auto launch = [&](auto kernel, const auto* p) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p, rows, K, ld, R, S, codes, scales); };
+    if (type == UITK_T_F32) split ? launch(mx4_quantize_kernel<float, true>, (const float*)x) : launch(mx4_quantize_kernel<float, false>, (const float*)x);
+    else if (type == UITK_T_F16) split ? launch(mx4_quantize_kernel<_Float16, true>, (const _Float16*)x) : launch(mx4_quantize_kernel<_Float16, false>, (const _Float16*)x);
+    else split ? launch(mx4_quantize_kernel<__bf16, true>, (const __bf16*)x) : launch(mx4_quantize_kernel<__bf16, false>, (const __bf16*)x);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }
@@ -642,6 +668,7 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     if (rows == 0) return UITK_OK;
     if (!x || !q) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_dequantize: null pointer");
     if (ld < K) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_dequantize: rows overlap (ld < K)");
+    if (!on_element(x, type)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_dequantize: x is not aligned to its elements");
     if (!aligned16(q)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_dequantize: the packed buffer must be 16-byte aligned");
     const int64_t R = (rows + MX4_ROWS - 1) / MX4_ROWS, S = (K + MX4_K - 1) / MX4_K;
     if ((R * S + 3) / 4 > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_dequantize: more elements than one launch takes");
@@ -673,6 +700,9 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     if (!u->x || !u->w || !u->out) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: null pointer");
     if (!aligned16(u->w) || (u->x_type == UITK_T_MX4 && !aligned16(u->x)) || (u->out_type == UITK_T_MX4 && !aligned16(u->out)))
         return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: packed matrices must be 16-byte aligned");
+    if (!on_element(u->bias, UITK_T_F32) || (u->x_type != UITK_T_MX4 && !on_element(u->x, u->x_type)) ||
+        (u->out_type != UITK_T_MX4 && (!on_element(u->out, u->out_type) || !on_element(u->residual, u->out_type))))
+        return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: a pointer is not aligned to its elements");
     if (u->x_type != UITK_T_MX4 && u->ldx < u->K) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: rows of x overlap (ldx < K)");
     if (u->out_type != UITK_T_MX4 && u->ldo < u->N) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: rows of the output overlap (ldo < N)");
     if (u->residual && u->ldr < u->N) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: rows of the residual overlap (ldr < N)");

@@ -32,7 +32,7 @@ typedef __bf16 mx_b2 __attribute__((ext_vector_type(2)));
 typedef unsigned mx_u4 __attribute__((ext_vector_type(4)));
 typedef unsigned mx_u2 __attribute__((ext_vector_type(2)));
 // the same at the alignment of their elements: global memory takes 16-byte accesses at any address, so a row that starts anywhere (an odd
-// width, a slice) still goes 16 bytes a lane (quantize 32768 x 4095 bf16, element by element / like this: 453 / 137 us; 4096 wide: 75)
+// width, a slice) still goes 16 bytes a lane (quantize 32768 x 4095 bf16, element by element / like this: 453 / 102 us; 4096 wide: 72)
 typedef unsigned mx_u4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned mx_u2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef float mx_f4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -145,6 +145,59 @@ template <> struct Mx4Src<__bf16> : Mx4Src16<__bf16> {
     }
 };
 
+// ---- 8 elements of a row, four neighbouring lanes a block
+template <typename T> struct Mx4Oct;
+template <> struct Mx4Oct<float> {
+    mx_f4 v[2];
+    __device__ __forceinline__ void load(const float* p, int n) {                           // n valid elements (0 or less: none)
+        if (n >= 8) { v[0] = ((const mx_f4u*)p)[0]; v[1] = ((const mx_f4u*)p)[1]; return; }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = i < n ? p[i] : 0.f;
+    }
+    __device__ __forceinline__ unsigned exponent() const;                                   // of the block's largest magnitude, as a float32 exponent field
+    __device__ __forceinline__ unsigned pack(float s) const {
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0][0], v[0][1], s, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0][2], v[0][3], s, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[1][0], v[1][1], s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[1][2], v[1][3], s, 3);
+    }
+};
+template <typename T> struct Mx4Oct16 {
+    mx_u4 v;
+    __device__ __forceinline__ void load(const T* p, int n) {
+        if (n >= 8) { v = *(const mx_u4u*)p; return; }
+        const unsigned short* q = (const unsigned short*)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (2 * i < n ? (unsigned)q[2 * i] : 0u) | (2 * i + 1 < n ? (unsigned)q[2 * i + 1] << 16 : 0u);
+    }
+    __device__ __forceinline__ unsigned amax() const;                                       // the 15 bits of the block's largest magnitude
+};
+template <> struct Mx4Oct<_Float16> : Mx4Oct16<_Float16> {
+    __device__ __forceinline__ unsigned exponent() const { return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)amax())) >> 23; }
+    __device__ __forceinline__ unsigned pack(float s) const {
+        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+        const h8 h = __builtin_bit_cast(h8, v);
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, mx_h2{h[0], h[1]}, s, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, mx_h2{h[2], h[3]}, s, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, mx_h2{h[4], h[5]}, s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, mx_h2{h[6], h[7]}, s, 3);
+    }
+};
+template <> struct Mx4Oct<__bf16> : Mx4Oct16<__bf16> {
+    __device__ __forceinline__ unsigned exponent() const { return amax() >> 7; }
+    __device__ __forceinline__ unsigned pack(float s) const {
+        typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+        const b8 h = __builtin_bit_cast(b8, v);
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_b2{h[0], h[1]}, s, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_b2{h[2], h[3]}, s, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_b2{h[4], h[5]}, s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, mx_b2{h[6], h[7]}, s, 3);
+    }
+};
+
 // ---- reductions over neighbouring lanes without LDS: DPP within 16 lanes, row swaps beyond
 template <int CTRL> __device__ __forceinline__ unsigned mx_dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
@@ -162,6 +215,20 @@ template <int N, typename F> __device__ __forceinline__ unsigned mx_lanes(unsign
 template <int N> __device__ __forceinline__ unsigned mx_lanes_max(unsigned v) { return mx_lanes<N>(v, [](unsigned a, unsigned b) { return max(a, b); }); }
 template <int N> __device__ __forceinline__ float mx_lanes_sum(float v) {
     return __uint_as_float(mx_lanes<N>(__float_as_uint(v), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+
+__device__ __forceinline__ unsigned Mx4Oct<float>::exponent() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i >> 2][i & 3]) & 0x7fffffffu);
+    return mx_lanes_max<4>(m) >> 23;
+}
+template <typename T> __device__ __forceinline__ unsigned Mx4Oct16<T>::amax() const {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    us2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const unsigned a = v[i] & 0x7fff7fffu; m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, a)); }
+    return mx_lanes_max<4>(max((unsigned)m[0], (unsigned)m[1]));
 }
 
 // ---- packing inside an epilogue: 8 neighbouring lanes hold 4 consecutive elements of a block each.  -> the lane's two bytes of codes

@@ -99,20 +99,29 @@ def _workspace_bytes(M, N, K, x_type):
     return _lib.load().uitk_mx4_linear_workspace(M, N, K, x_type)
 
 
+def _packed_bytes(shape):
+    rows, K = math.prod(shape[:-1]), shape[-1]
+    if rows > _MAX_ROWS or not 1 <= K <= _MAX_K:
+        raise ValueError(f"a packed 4-bit matrix of {rows} rows x {K} is out of range (rows <= 2^31, 1 <= K <= 2^20)")
+    return (rows + 63) // 64 * ((K + 127) // 128) * _RECORD_BYTES
+
+
 class Mx4Tensor:
     """A packed 4-bit matrix: `shape` is the logical shape (blocks run along the last dimension), `data` the packed bytes -- an opaque
     order made for the matrix pipe (csrc/mx4_dev.h)."""
 
     def __init__(self, data, shape):
-        self.data = data
-        self.shape = torch.Size(shape)
+        shape = torch.Size(shape)
+        if (not isinstance(data, torch.Tensor) or not data.is_cuda or data.dtype is not torch.uint8 or data.dim() != 1 or not data.is_contiguous()
+                or len(shape) < 1 or data.numel() != _packed_bytes(shape) or data.data_ptr() % 16):
+            raise ValueError(f"data must be the {_packed_bytes(shape) if len(shape) else 0} packed bytes of a {tuple(shape)} matrix: a contiguous, 16-byte aligned uint8 CUDA tensor")
+        self.data, self.shape = data, shape
 
     @classmethod
     def empty(cls, shape, device):
-        rows, K = math.prod(shape[:-1]), shape[-1]
-        if rows > _MAX_ROWS or not 1 <= K <= _MAX_K:
-            raise ValueError(f"a packed 4-bit matrix of {rows} rows x {K} is out of range (rows <= 2^31, 1 <= K <= 2^20)")
-        return cls(torch.empty((rows + 63) // 64 * ((K + 127) // 128) * _RECORD_BYTES, dtype=torch.uint8, device=device), shape)
+        q = cls.__new__(cls)
+        q.data, q.shape = torch.empty(_packed_bytes(shape), dtype=torch.uint8, device=device), torch.Size(shape)
+        return q
 
     @property
     def device(self):
