@@ -74,7 +74,7 @@ def test_refusals_before_any_launch():
         a = dict(x=1 << 20, w=1 << 21, out=1 << 22, M=4, N=8, K=32, ldx=32, ldo=8, x_type=0, out_type=0)
         a.update(kw)
         return L.uitk_mx4_linear(ctypes.byref(_lib.Mx4LinearArgs(**a)), None)
-    for kw in (dict(x=None), dict(w=None), dict(out=None), dict(N=0), dict(K=0), dict(M=-1), dict(x_type=4), dict(out_type=-1), dict(act=3), dict(ldx=31), dict(ldo=7),
+    for kw in (dict(x=None), dict(w=None), dict(out=None), dict(N=0), dict(K=0), dict(M=-1), dict(x_type=4), dict(out_type=-1), dict(act=3), dict(reserved=1), dict(ldx=31), dict(ldo=7),
                dict(w=(1 << 21) + 4), dict(residual=1 << 23, ldr=7), dict(residual=1 << 23, ldr=8, out_type=3), dict(x_type=3, x=(1 << 20) + 8),
                dict(out_type=3, out=(1 << 22) + 8)):
         assert call(**kw) == bad, kw

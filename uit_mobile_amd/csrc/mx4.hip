@@ -65,10 +65,10 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
 }
 
 // One wave per record here too; a lane turns the codes of 16 bytes of output into them, so that neighbouring lanes store neighbouring
-// bytes of a row (a whole block per lane would store 16-byte pieces 64 or 128 bytes apart: 32768 x 4096 bf16 750 / 73 us, 4.7 TB/s).
+// bytes of a row (a whole block per lane stored 16-byte pieces 64 or 128 bytes apart; 32768 x 4096 bf16: 56 us, 6.1 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales, int64_t rows, int64_t K, int64_t ld,
-                                                             int64_t R, int64_t S, T* __restrict__ x) {
+                                                             int64_t R, int64_t S, int stream, T* __restrict__ x) {
     constexpr int P = 16 / sizeof(T), LPR = MX4_K / P, RPI = 64 / LPR;      // elements of a lane, lanes of a row, rows at a time
     typedef T TP __attribute__((ext_vector_type(P)));
     typedef T TPu __attribute__((ext_vector_type(P), aligned(sizeof(T))));
@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restr
             if (r >= nrow) continue;
             T* o = x + (rg * MX4_ROWS + r) * ld + k;
             if (n == P) {
-                *(TPu*)o = t;
+                if (stream) __builtin_nontemporal_store(t, (TPu*)o);
+                else *(TPu*)o = t;
             } else {
 #pragma unroll
                 for (int j = 0; j < P - 1; ++j) if (j < n) o[j] = t[j];
@@ -143,6 +144,7 @@ template <> struct Mx4Out<MT_F32> {
     typedef float T;
     static __device__ __forceinline__ void add4(float (&v)[4], const float* r) { const mx_f4 t = *(const mx_f4u*)r; v[0] += t[0]; v[1] += t[1]; v[2] += t[2]; v[3] += t[3]; }
     static __device__ __forceinline__ void put4(float* o, const float (&v)[4]) { *(mx_f4u*)o = mx_f4{v[0], v[1], v[2], v[3]}; }
+    static __device__ __forceinline__ void stream4(float* o, const float (&v)[4]) { __builtin_nontemporal_store(mx_f4{v[0], v[1], v[2], v[3]}, (mx_f4u*)o); }
 };
 template <> struct Mx4Out<MT_F16> {
     typedef _Float16 T;
@@ -151,10 +153,12 @@ template <> struct Mx4Out<MT_F16> {
         const h4 t = *(const h4*)r;
         v[0] += (float)t[0]; v[1] += (float)t[1]; v[2] += (float)t[2]; v[3] += (float)t[3];
     }
-    static __device__ __forceinline__ void put4(_Float16* o, const float (&v)[4]) {
+    static __device__ __forceinline__ mx_u2 pack4(const float (&v)[4]) {
         const mx_h2 a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
-        *(mx_u2u*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+        return mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
     }
+    static __device__ __forceinline__ void put4(_Float16* o, const float (&v)[4]) { *(mx_u2u*)o = pack4(v); }
+    static __device__ __forceinline__ void stream4(_Float16* o, const float (&v)[4]) { __builtin_nontemporal_store(pack4(v), (mx_u2u*)o); }
 };
 template <> struct Mx4Out<MT_BF16> {
     typedef __bf16 T;
@@ -162,10 +166,12 @@ template <> struct Mx4Out<MT_BF16> {
         const mx_u2 t = *(const mx_u2u*)r;
         v[0] += __uint_as_float(t[0] << 16); v[1] += __uint_as_float(t[0] & 0xffff0000u); v[2] += __uint_as_float(t[1] << 16); v[3] += __uint_as_float(t[1] & 0xffff0000u);
     }
-    static __device__ __forceinline__ void put4(__bf16* o, const float (&v)[4]) {
+    static __device__ __forceinline__ mx_u2 pack4(const float (&v)[4]) {
         const mx_b2 a = {(__bf16)v[0], (__bf16)v[1]}, b = {(__bf16)v[2], (__bf16)v[3]};
-        *(mx_u2u*)o = mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+        return mx_u2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
     }
+    static __device__ __forceinline__ void put4(__bf16* o, const float (&v)[4]) { *(mx_u2u*)o = pack4(v); }
+    static __device__ __forceinline__ void stream4(__bf16* o, const float (&v)[4]) { __builtin_nontemporal_store(pack4(v), (mx_u2u*)o); }
 };
 // n of the four are inside the row
 template <int OUT>
@@ -381,7 +387,7 @@ __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const flo
             for (int i = 0; i < 4; ++i) v[i] = mx4_act<ACT>(w[i] + bias[i]);
             if (whole) {
                 if (a.residual) Mx4Out<OUT>::add4(v, (const T*)a.residual + r);
-                Mx4Out<OUT>::put4((T*)a.out + o, v);
+                Mx4Out<OUT>::stream4((T*)a.out + o, v);                    // (streamed past the caches: 4 to 10 % of a call whose K is narrow)
             } else if (it * RPI + row < rows && in > 0) {
                 mx4_finish4<OUT>(a.out, o, a.residual, r, in, v);
             }
@@ -676,9 +682,11 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     const char* scales = codes + R * S * MX4_CODES;
     const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (float*)x);
-    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_dequantize_kernel<_Float16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (_Float16*)x);
-    else hipLaunchKernelGGL(mx4_dequantize_kernel<__bf16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, (__bf16*)x);
+    // whole 16-byte pieces go past the caches (32768 x 4096 bf16 73 / 56 us), pieces across their borders must not (4095 wide: 104 / 126)
+    const int nt = aligned16(x) && ld * (type == UITK_T_F32 ? 4 : 2) % 16 == 0;
+    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (float*)x);
+    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_dequantize_kernel<_Float16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (_Float16*)x);
+    else hipLaunchKernelGGL(mx4_dequantize_kernel<__bf16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (__bf16*)x);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }
@@ -696,6 +704,7 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     if (u->out_type < UITK_T_F32 || u->out_type > UITK_T_MX4) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: unknown out_type");
     if (u->act < 0 || u->act > 2) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: act must be 0 (none), 1 (ReLU) or 2 (GELU)");
     if (u->residual && u->out_type == UITK_T_MX4) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: a residual needs an output of 16 or 32 bits");
+    if (u->reserved) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: reserved must be 0");
     if (u->M == 0) return UITK_OK;
     if (!u->x || !u->w || !u->out) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: null pointer");
     if (!aligned16(u->w) || (u->x_type == UITK_T_MX4 && !aligned16(u->x)) || (u->out_type == UITK_T_MX4 && !aligned16(u->out)))
@@ -715,12 +724,7 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     a.out = u->out; a.ldo = u->ldo; a.out_type = u->out_type;
     if (u->out_type == UITK_T_MX4) { a.out_S = (u->N + MX4_K - 1) / MX4_K; a.out_scales = (char*)u->out + mx4_records(u->M, u->N) * MX4_CODES; }
     hipStream_t s = (hipStream_t)stream;
-#ifdef UITK_LAB
-    Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
-    if (u->reserved) { plan.kernel = u->reserved - 1; plan.quantize_first = u->x_type != UITK_T_MX4 && plan.kernel >= MX4_TILE128; }
-#else
     const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
-#endif
     if (plan.quantize_first) {
         if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
         if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
