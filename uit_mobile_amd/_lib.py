@@ -127,7 +127,15 @@ def load():
     return L
 
 
-_packed = {}
+_packed, _entries = {}, {}
+
+
+def entry(name):
+    """The entry point `name`, looked up once."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    return fn
 
 
 def packed(name):

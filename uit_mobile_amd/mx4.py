@@ -32,9 +32,12 @@ def run(fn, device, *args):
     i = device.index
     stream = torch._C._cuda_getCurrentRawStream(i)
     if torch._C._cuda_getDevice() == i:
-        return _lib.check(fn(*args, stream), fn.__name__)
-    with torch.cuda.device(i):
-        _lib.check(fn(*args, stream), fn.__name__)
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, fn.__name__)
 
 
 def check_tensor(t, name):
@@ -99,8 +102,7 @@ def _workspace_bytes(M, N, K, x_type):
     return _lib.load().uitk_mx4_linear_workspace(M, N, K, x_type)
 
 
-def _packed_bytes(shape):
-    rows, K = math.prod(shape[:-1]), shape[-1]
+def _packed_bytes(rows, K):
     if rows > _MAX_ROWS or not 1 <= K <= _MAX_K:
         raise ValueError(f"a packed 4-bit matrix of {rows} rows x {K} is out of range (rows <= 2^31, 1 <= K <= 2^20)")
     return (rows + 63) // 64 * ((K + 127) // 128) * _RECORD_BYTES
@@ -112,15 +114,19 @@ class Mx4Tensor:
 
     def __init__(self, data, shape):
         shape = torch.Size(shape)
+        if not shape:
+            raise ValueError("a packed matrix has at least one dimension")
+        need = _packed_bytes(math.prod(shape[:-1]), shape[-1])
         if (not isinstance(data, torch.Tensor) or not data.is_cuda or data.dtype is not torch.uint8 or data.dim() != 1 or not data.is_contiguous()
-                or len(shape) < 1 or data.numel() != _packed_bytes(shape) or data.data_ptr() % 16):
-            raise ValueError(f"data must be the {_packed_bytes(shape) if len(shape) else 0} packed bytes of a {tuple(shape)} matrix: a contiguous, 16-byte aligned uint8 CUDA tensor")
+                or data.numel() != need or data.data_ptr() % 16):
+            raise ValueError(f"data must be the {need} packed bytes of a {tuple(shape)} matrix: a contiguous, 16-byte aligned uint8 CUDA tensor")
         self.data, self.shape = data, shape
 
     @classmethod
-    def empty(cls, shape, device):
+    def empty(cls, shape, device, rows=None):
         q = cls.__new__(cls)
-        q.data, q.shape = torch.empty(_packed_bytes(shape), dtype=torch.uint8, device=device), torch.Size(shape)
+        q.shape = shape = torch.Size(shape)
+        q.data = torch.empty(_packed_bytes(math.prod(shape[:-1]) if rows is None else rows, shape[-1]), dtype=torch.uint8, device=device)
         return q
 
     @property
@@ -144,20 +150,22 @@ class Mx4Tensor:
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         if out.numel():
             K = self.shape[-1]
-            run(_lib.load().uitk_mx4_dequantize, out.device, self.data.data_ptr(), out.numel() // K, K, out.data_ptr(), _TYPES[dtype], K)
+            run(_lib.entry("uitk_mx4_dequantize"), out.device, self.data.data_ptr(), out.numel() // K, K, out.data_ptr(), _TYPES[dtype], K)
         return out
 
 
 def quantize(x):
     """x [..., K] (float32 / float16 / bfloat16) -> Mx4Tensor of the same shape."""
     code = check_tensor(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be [..., K] with K >= 1, got {tuple(x.shape)}")
-    q = Mx4Tensor.empty(x.shape, x.device)
-    if x.numel():
-        K = x.shape[-1]
+    shape, device = x.shape, x.device
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"x must be [..., K] with K >= 1, got {tuple(shape)}")
+    K = shape[-1]
+    rows = x.numel() // K
+    q = Mx4Tensor.empty(shape, device, rows)
+    if rows:
         v, ld = as_rows(x, K)
-        run(_lib.load().uitk_mx4_quantize, x.device, v.data_ptr(), code, x.numel() // K, K, ld, q.data.data_ptr())
+        run(_lib.entry("uitk_mx4_quantize"), device, v.data_ptr(), code, rows, K, ld, q.data.data_ptr())
     return q
 
 
@@ -214,7 +222,7 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
         if residual is not None and overlaps(mine, span(residual)) and not (out.data_ptr() == residual.data_ptr() and residual.is_contiguous()):
             raise ValueError("out shares memory with the residual without being the residual")
     if to_mx4:
-        result = Mx4Tensor.empty(shape, device)
+        result = Mx4Tensor.empty(shape, device, M)
         dst, out_type = result.data, _lib.T_MX4
     else:
         result = dst = new(shape, out_dtype, w.data if packed else x) if out is None else out

@@ -78,7 +78,7 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
     h, h_type, h_ptr = None, 0, 0
     if pre is not None:
         if out_dtype == "mx4":
-            h, h_type = Mx4Tensor.empty(shape, device), _lib.T_MX4
+            h, h_type = Mx4Tensor.empty(shape, device, rows), _lib.T_MX4
             h_ptr = h.data.data_ptr()
         elif out_dtype in _TYPES:
             h, h_type = new(shape, out_dtype, residual), _TYPES[out_dtype]
