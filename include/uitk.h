@@ -390,7 +390,7 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* a, void* stream);
 
 /* residual_out = residual + gate * scale * post(y);  h = pre(residual_out).  post / pre: LayerNorm or root mean square over D, in fp32; h is taken
  * from the unrounded sum.  y NULL: h = pre(residual) only (no post, gate, scale; residual_out is not written).
- * Stands in for the residual adds, LayerScale and norms of Block.forward (models/uit.py:244-247, 78-85). */
+ * Stands in for the residual adds, LayerScale and norms of Block.forward (models/uit.py:245-248, 78-85). */
 typedef enum uitk_norm { UITK_NORM_LAYER = 0, UITK_NORM_RMS = 1 } uitk_norm;
 typedef struct uitk_block_norm_args {
     const void* y;                         /* [rows, D] the block's output, or NULL */

@@ -5,7 +5,7 @@
 //     h  = pre(r')                      norm in front of the next block (optional), 32, 16 or 4 bits (mx4_dev.h)
 //
 // post / pre: LayerNorm ((v - mean) / sqrt(var + eps)) or root mean square (v / sqrt(mean(v^2) + eps)), then gain and offset (each optional).
-// All of it in fp32 from the inputs to the one rounding of each output; h is taken from the unrounded r'.  (models/uit.py:244-247: Block.forward,
+// All of it in fp32 from the inputs to the one rounding of each output; h is taken from the unrounded r'.  (models/uit.py:245-248: Block.forward,
 // whose LayerScale is :78-85.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -4,7 +4,7 @@
     r' = residual + gate * scale * z    gate per sequence or per token, scale per channel (LayerScale); both optional
     h  = pre(r')                        norm in front of the next block (optional)
 
-What Block.forward of the reference does in separate operations between two linears (models/uit.py:244-247).  fp32 arithmetic whatever the
+What Block.forward of the reference does in separate operations between two linears (models/uit.py:245-248).  fp32 arithmetic whatever the
 types, one rounding per output, h from the unrounded r'.  `UITBase(precision='mx4')` runs its blocks on it.  CUDA tensors only, enqueue-only
 on the tensors' device and its current stream, no gradients (a call that autograd would have to record is refused).
 """
