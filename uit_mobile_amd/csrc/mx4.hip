@@ -189,14 +189,19 @@ __device__ __forceinline__ void mx4_finish4(void* out, int64_t o, const void* re
     }
 }
 
+template <int ACT> __device__ __forceinline__ float mx4_act(float v) {
+    if constexpr (ACT == 1) return v < 0.f ? 0.f : v;                       // (a NaN stays one)
+    else if constexpr (ACT == 2) return mx4_gelu(v);
+    else return v;
+}
+
 // four consecutive outputs (row m, columns n ..): bias, activation, residual, one rounding, store
 __device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, int64_t n, const mx_f4& bias, float (&v)[4]) {
     const bool in_m = m < a.M;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[i] += bias[i];
-        if (a.act == 1) v[i] = v[i] > 0.f ? v[i] : (v[i] != v[i] ? v[i] : 0.f);              // a NaN stays one
-        else if (a.act == 2) v[i] = mx4_gelu(v[i]);
+        v[i] = a.act == 0 ? v[i] : a.act == 1 ? mx4_act<1>(v[i]) : mx4_act<2>(v[i]);
     }
     if (a.out_type == MT_MX4) {                                             // (8 neighbouring lanes hold one block: no divergence up to here)
 #pragma unroll
@@ -331,12 +336,6 @@ struct Mx4Tile {
 
 // ---- a wave's 32 tokens x 32 TN outputs, from its part of LDS to memory.  n0, m0: the first column / row; bias added, activation, residual
 // added, one rounding, four columns a lane.
-template <int ACT> __device__ __forceinline__ float mx4_act(float v) {
-    if constexpr (ACT == 1) return v < 0.f ? 0.f : v;                       // (a NaN stays one)
-    else if constexpr (ACT == 2) return mx4_gelu(v);
-    else return v;
-}
-
 template <int OUT, int COLS, int LDE, int ACT>
 __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const float* ep, int64_t m0, int64_t n0) {
     const int lane = threadIdx.x & 63;
@@ -396,7 +395,7 @@ __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const flo
 }
 
 template <int BN, int BM, int WN, int WM, int OUT>
-__global__ void __launch_bounds__(64 * WN * WM, BN * BM <= 256 * 128 ? 2 : 1) mx4_tile_kernel(Mx4LinearArgs a, int ntiles, int mtiles) {
+__global__ void __launch_bounds__(64 * WN * WM, 2) mx4_tile_kernel(Mx4LinearArgs a, int ntiles, int mtiles) {
     typedef Mx4Tile<BN, BM, WN, WM> T;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
