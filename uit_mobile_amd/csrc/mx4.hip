@@ -66,9 +66,9 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
 
 // One wave per record here too; a lane turns the codes of 16 bytes of output into them, so that neighbouring lanes store neighbouring
 // bytes of a row (a whole block per lane stored 16-byte pieces 64 or 128 bytes apart; 32768 x 4096 bf16: 56 us, 6.1 TB/s).
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales, int64_t rows, int64_t K, int64_t ld,
-                                                             int64_t R, int64_t S, int stream, T* __restrict__ x) {
+                                                             int64_t R, int64_t S, T* __restrict__ x) {
     constexpr int P = 16 / sizeof(T), LPR = MX4_K / P, RPI = 64 / LPR;      // elements of a lane, lanes of a row, rows at a time
     typedef T TP __attribute__((ext_vector_type(P)));
     typedef T TPu __attribute__((ext_vector_type(P), aligned(sizeof(T))));
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const char* __restr
             if (r >= nrow) continue;
             T* o = x + (rg * MX4_ROWS + r) * ld + k;
             if (n == P) {
-                if (stream) __builtin_nontemporal_store(t, (TPu*)o);
+                if constexpr (STREAM) __builtin_nontemporal_store(t, (TPu*)o);
                 else *(TPu*)o = t;
             } else {
 #pragma unroll
@@ -335,11 +335,10 @@ struct Mx4Tile {
 };
 
 // ---- a wave's 32 tokens x 32 TN outputs, from its part of LDS to memory.  n0, m0: the first column / row; bias added, activation, residual
-// added, one rounding, four columns a lane.
+// added, one rounding, 16 bytes of output a lane (16-bit outputs, 8 bytes / 16 a lane: 16128 x 2304 x 768 29 / 27.5 us).
 template <int OUT, int COLS, int LDE, int ACT>
 __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const float* ep, int64_t m0, int64_t n0) {
     const int lane = threadIdx.x & 63;
-    constexpr int LPR = COLS / 4, RPI = 64 / LPR;                           // lanes that hold a row, rows an instruction stores
     if constexpr (OUT == MT_MX4) {
         // eight columns a lane, four lanes a block; m0 is a multiple of 32, so a lane's blocks lie 16 bytes a row apart
         constexpr int L8 = COLS / 8, R8 = 64 / L8;
@@ -372,23 +371,38 @@ __device__ __forceinline__ void mx4_store_tile(const Mx4LinearArgs& a, const flo
     } else {
         typedef typename Mx4Out<OUT>::T T;
         if (m0 >= a.M || n0 >= a.N) return;
-        const int64_t n = n0 + (lane % LPR) * 4;
-        const mx_f4 bias = mx4_bias4(a, n);
-        const int row = lane / LPR, in = (int)min((int64_t)4, a.N - n);
+        // as many columns a lane as 16 bytes of output hold
+        constexpr int C = 16 / sizeof(T), LR = COLS / C, RI = 64 / LR;
+        const int64_t n = n0 + (lane % LR) * C;
+        const int row = lane / LR, in = (int)min((int64_t)C, a.N - n);
+        mx_f4 bias[C / 4];
+#pragma unroll
+        for (int q = 0; q < C / 4; ++q) bias[q] = mx4_bias4(a, n + 4 * q);
         int64_t o = (m0 + row) * a.ldo + n, r = (m0 + row) * a.ldr + n;
         const bool whole = n0 + COLS <= a.N && m0 + 32 <= a.M;              // (of the wave)
         const int rows = (int)min((int64_t)32, a.M - m0);
-#pragma unroll 4
-        for (int it = 0; it < 32 / RPI; ++it, o += RPI * a.ldo, r += RPI * a.ldr) {
-            const mx_f4 w = *(const mx_f4*)&ep[(it * RPI + row) * LDE + (lane % LPR) * 4];
-            float v[4];
+#pragma unroll 2
+        for (int it = 0; it < 32 / RI; ++it, o += RI * a.ldo, r += RI * a.ldr) {
+            float v[C / 4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = mx4_act<ACT>(w[i] + bias[i]);
+            for (int q = 0; q < C / 4; ++q) {
+                const mx_f4 w = *(const mx_f4*)&ep[(it * RI + row) * LDE + (lane % LR) * C + 4 * q];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[q][i] = mx4_act<ACT>(w[i] + bias[q][i]);
+            }
             if (whole) {
-                if (a.residual) Mx4Out<OUT>::add4(v, (const T*)a.residual + r);
-                Mx4Out<OUT>::stream4((T*)a.out + o, v);                    // (streamed past the caches: 4 to 10 % of a call whose K is narrow)
-            } else if (it * RPI + row < rows && in > 0) {
-                mx4_finish4<OUT>(a.out, o, a.residual, r, in, v);
+                if (a.residual) {
+#pragma unroll
+                    for (int q = 0; q < C / 4; ++q) Mx4Out<OUT>::add4(v[q], (const T*)a.residual + r + 4 * q);
+                }
+                if constexpr (C == 4) Mx4Out<OUT>::stream4((T*)a.out + o, v[0]);
+                else {
+                    const mx_u2 lo = Mx4Out<OUT>::pack4(v[0]), hi = Mx4Out<OUT>::pack4(v[C / 4 - 1]);
+                    __builtin_nontemporal_store(mx_u4{lo[0], lo[1], hi[0], hi[1]}, (mx_u4u*)((T*)a.out + o));
+                }
+            } else if (it * RI + row < rows) {
+#pragma unroll
+                for (int q = 0; q < C / 4; ++q) if (in > 4 * q) mx4_finish4<OUT>(a.out, o + 4 * q, a.residual, r + 4 * q, in - 4 * q, v[q]);
             }
         }
     }
@@ -682,10 +696,11 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
     const dim3 grid((unsigned)((R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
     // whole 16-byte pieces go past the caches (32768 x 4096 bf16 73 / 56 us), pieces across their borders must not (4095 wide: 104 / 126)
-    const int nt = aligned16(x) && ld * (type == UITK_T_F32 ? 4 : 2) % 16 == 0;
-    if (type == UITK_T_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (float*)x);
-    else if (type == UITK_T_F16) hipLaunchKernelGGL(mx4_dequantize_kernel<_Float16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (_Float16*)x);
-    else hipLaunchKernelGGL(mx4_dequantize_kernel<__bf16>, grid, block, 0, s, codes, scales, rows, K, ld, R, S, nt, (__bf16*)x);
+    const bool nt = aligned16(x) && ld * (type == UITK_T_F32 ? 4 : 2) % 16 == 0;
+    auto launch = [&](auto kernel, auto* p) { hipLaunchKernelGGL(kernel, grid, block, 0, s, codes, scales, rows, K, ld, R, S, p); };
+    if (type == UITK_T_F32) nt ? launch(mx4_dequantize_kernel<float, true>, (float*)x) : launch(mx4_dequantize_kernel<float, false>, (float*)x);
+    else if (type == UITK_T_F16) nt ? launch(mx4_dequantize_kernel<_Float16, true>, (_Float16*)x) : launch(mx4_dequantize_kernel<_Float16, false>, (_Float16*)x);
+    else nt ? launch(mx4_dequantize_kernel<__bf16, true>, (__bf16*)x) : launch(mx4_dequantize_kernel<__bf16, false>, (__bf16*)x);
     MX4_HIP(hipGetLastError());
     return UITK_OK;
 }
