@@ -87,8 +87,10 @@ def check_vector(t, name, n, device, keep):
     """A per-channel parameter: [n] on `device` -> the address of its values in float32 (0: None).  What had to be converted joins `keep`."""
     if t is None:
         return 0
-    if check_tensor(t, name) == _lib.T_F32 and t.get_device() == device.index and t.dim() == 1 and t.numel() == n and t.is_contiguous():
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device.index and t.dim() == 1 and t.numel() == n
+            and t.is_contiguous() and not (t.requires_grad and torch.is_grad_enabled())):
         return t.data_ptr()
+    check_tensor(t, name)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
     if t.device != device:
