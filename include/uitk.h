@@ -377,8 +377,8 @@ typedef struct uitk_mx4_linear_args {
     const void* x;         /* [M, K], rows ldx elements apart; or packed */
     const void* w;         /* packed [N, K] */
     const float* bias;     /* [N] or NULL */
-    const void* residual;  /* [M, N] of out_type, rows ldr apart, or NULL; may be `out` itself */
-    void* out;             /* [M, N], rows ldo apart; or packed */
+    const void* residual;  /* [M, N] of out_type, rows ldr apart, or NULL; may be `out` itself (ldr == ldo) */
+    void* out;             /* [M, N], rows ldo apart; or packed.  Shares no memory with an input, but for a residual that is `out` */
     void* workspace;       /* uitk_mx4_linear_workspace bytes, 16-byte aligned, of this call until it has run (NULL when 0) */
     int64_t M, N, K, ldx, ldr, ldo;
     int32_t x_type, out_type; /* uitk_type */
@@ -395,7 +395,7 @@ typedef enum uitk_norm { UITK_NORM_LAYER = 0, UITK_NORM_RMS = 1 } uitk_norm;
 typedef struct uitk_block_norm_args {
     const void* y;                         /* [rows, D] the block's output, or NULL */
     const void* residual;                  /* [rows, D] */
-    void* residual_out;                    /* [rows, D] of r_type; may be `residual` itself */
+    void* residual_out;                    /* [rows, D] of r_type; may be `residual` itself (ldro == ldr); outputs share no other memory */
     void* h;                               /* [rows, D] of h_type, or packed (UITK_T_MX4); may be `y` itself where type and rows agree */
     const void* gate;                      /* row m of the stream uses gate row m / gate_rows: 1 = per token, T = per sequence; or NULL */
     const float* scale;                    /* [D] or NULL */

@@ -405,6 +405,12 @@ def test_packed_matrices_are_checked_where_they_are_made():
             mx4.Mx4Tensor(data, shape)
 
 
+@pytest.mark.parametrize("shape", [(), (-1, 32), (-64, -1, 32), (64, -32)])
+def test_packed_shapes_without_a_meaning(shape):
+    with pytest.raises(ValueError, match="at least one dimension and none below zero"):
+        mx4.Mx4Tensor(None, shape)
+
+
 @gpu
 def test_offsets_past_32_bits():
     """More than 2^31 elements: the last rows of a large call are those of a small one."""

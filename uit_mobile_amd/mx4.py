@@ -116,8 +116,8 @@ class Mx4Tensor:
 
     def __init__(self, data, shape):
         shape = torch.Size(shape)
-        if not shape:
-            raise ValueError("a packed matrix has at least one dimension")
+        if not shape or min(shape) < 0:
+            raise ValueError(f"a packed matrix has at least one dimension and none below zero, got {tuple(shape)}")
         need = _packed_bytes(math.prod(shape[:-1]), shape[-1])
         if (not isinstance(data, torch.Tensor) or not data.is_cuda or data.dtype is not torch.uint8 or data.dim() != 1 or not data.is_contiguous()
                 or data.numel() != need or data.data_ptr() % 16):
