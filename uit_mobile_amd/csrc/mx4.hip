@@ -13,6 +13,7 @@
 
 #include "../../include/uitk.h"
 #include "mx4_dev.h"
+#include "mx4_plan.h"
 
 namespace uitk {
 
@@ -611,27 +612,6 @@ static hipError_t mx4_launch_rows(Mx4LinearArgs& a, hipStream_t s) {
     return go(mx4_rows_kernel<NT, NW, __bf16, false>);
 }
 
-// Which kernel, and whether activations that are not packed are quantised inside it.  us on the GPU, packed x unless said otherwise:
-// * rows against tiles: 128 x 128 tiles need more than 128 of them (rows / 128 x 128: 512 x 4096 x 4096: 12.5 / 13.1; 128 x 16384 x 4096: 15.7 / 19.2;
-//   300 x 8192 x 512: 7.7 / 6.1; 2048 x 4096 x 2048: 31 / 16), 256 x 128 ones two workgroups on every CU and a K that outweighs their longer
-//   epilogue (128 x 128 / 256 x 128: 16128 x 2304 x 768: 28.7 / 36.8; 16128 x 2304 x 2048: 50.4 / 55.2; 4096 x 4096 x 4096: 41.3 / 40.1; 8192 x 8192 x 8192: 270 / 254).
-// * rows: 8 waves share K, 16 where a wave would still have two records or more (13 x 8192 x 8192, 8 / 16: 12.5 / 11.9); with more than 512
-//   workgroups 64 columns each instead of 32 (128 x 8192 x 8192, 32 / 64: 21.4 / 17.5).
-// * quantising inside repeats the work in every column group, about 65 vector instructions per 32 x 64 fragment; a launch of its own costs
-//   2.6 us of the GPU, and a caller that does not replay a graph 3 us of the host and a workspace.  bf16 inside / packed, GPU: 1 x 2304 x 768 (864
-//   fragments) 4.4 / 3.2, 252 x 768 x 768 (2304) 4.9 / 3.4, 1003 x 537 x 1000 (8704) 11 / 5.1, 64 x 4096 x 4096 (16384) 12.4 / 6.0, 13 x 8192 x 8192 (32768) 17.7 / 11.9.
-enum { MX4_ROWS8 = 0, MX4_ROWS16, MX4_ROWS64, MX4_TILE128, MX4_TILE256 };
-struct Mx4Plan { int kernel; bool quantize_first; };
-static Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t K, int x_type) {
-    const int64_t m128 = (M + 127) / 128, S = (K + MX4_K - 1) / MX4_K, groups = ((N + 31) / 32) * ((M + 31) / 32);
-    Mx4Plan p{MX4_ROWS8, x_type != MT_MX4};
-    if (M > 64 && m128 * ((N + 127) / 128) > 128) p.kernel = m128 * ((N + 255) / 256) >= 512 && K >= 4096 ? MX4_TILE256 : MX4_TILE128;
-    else if (groups > 512) p.kernel = MX4_ROWS64;
-    else if (S >= 32) p.kernel = MX4_ROWS16;
-    if (p.kernel < MX4_TILE128 && 2 * groups * S <= 10240) p.quantize_first = false;
-    return p;
-}
-
 template <int BN, int BM, int WN, int WM, int OUT>
 static hipError_t mx4_launch_tile_as(const Mx4LinearArgs& a, hipStream_t s) {
     typedef Mx4Tile<BN, BM, WN, WM> T;
@@ -707,7 +687,7 @@ int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int typ
 
 int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type) {
     if (M < 0 || M > MX4_MAX_ROWS || N < 1 || N > MX4_MAX_K || K < 1 || K > MX4_MAX_K || x_type < UITK_T_F32 || x_type > UITK_T_MX4) return -1;
-    return mx4_plan(M, N, K, x_type).quantize_first ? mx4_bytes(M, K) : 0;
+    return mx4_plan(M, N, K, x_type == UITK_T_MX4).quantize_first ? mx4_bytes(M, K) : 0;
 }
 
 int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
@@ -738,7 +718,7 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     a.out = u->out; a.ldo = u->ldo; a.out_type = u->out_type;
     if (u->out_type == UITK_T_MX4) { a.out_S = (u->N + MX4_K - 1) / MX4_K; a.out_scales = (char*)u->out + mx4_records(u->M, u->N) * MX4_CODES; }
     hipStream_t s = (hipStream_t)stream;
-    const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type);
+    const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type == UITK_T_MX4);
     if (plan.quantize_first) {
         if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
         if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
