@@ -372,7 +372,7 @@ int uitk_mx4_quantize(const void* x, int type, int64_t rows, int64_t K, int64_t 
 int uitk_mx4_dequantize(const void* q, int64_t rows, int64_t K, void* x, int type, int64_t ld, void* stream);
 
 /* out[M, N] = residual + act(Q(x) . W^T + bias): Q(x) the 4-bit rounding of x [M, K] (or x packed already: x_type UITK_T_MX4), W packed [N, K].
- * Products are exact, sums are fp32, the output is rounded once.  out_type UITK_T_MX4: `out` is a packed [M, N] matrix -- the next layer's x. */
+ * Products are exact, sums are fp32 (in an order that may differ between calls of different sizes), the output is rounded once.  out_type UITK_T_MX4: `out` is a packed [M, N] matrix -- the next layer's x. */
 typedef struct uitk_mx4_linear_args {
     const void* x;         /* [M, K], rows ldx elements apart; or packed */
     const void* w;         /* packed [N, K] */

@@ -29,6 +29,7 @@
 
 #include "../../include/uitk.h"
 #include "mx4_dev.h"
+#include "mx4_plan.h"
 #include "naive_forward.h"
 #include "uitk_dev.h"
 
@@ -674,7 +675,8 @@ static hipError_t gen_attention(const float* QKV, float* O, int n, const GenGeom
 
 // precision 'mx4': the blocks of n clip-crops and the final norm.  R: the fp32 residual stream; Xn receives the blocks' outputs on their
 // way into it and, last, norm(R) for the head.  Every dense layer reads 4-bit activations: the norms and the MLP's first layer write
-// them, the attention's output is rounded by its product.
+// them, the attention's output is rounded by its product.  Norms and attention take a row or a clip by itself, and the products run on the
+// kernels that add in one order whatever the number of rows: a clip's result is the same in any batch, shard or chunk.
 static int gen_blocks_mx4(uitk_general* m, const GenGeom& g, int n, float* R, float* Xn, float* QKV, float* O, float scale, hipStream_t s) {
     const int64_t M = (int64_t)n * g.ntok;
     const GenWork4 w4 = gen_work4(g, M);
@@ -694,7 +696,7 @@ static int gen_blocks_mx4(uitk_general* m, const GenGeom& g, int n, float* R, fl
         uitk_mx4_linear_args a{};
         a.x = x; a.x_type = x_type; a.ldx = K; a.w = m->packed + m->packed_off[4 * (size_t)b + layer]; a.bias = bias; a.act = act; a.out = out; a.out_type = out_type;
         a.ldo = N; a.M = M; a.N = N; a.K = K; a.workspace = att;
-        return uitk_mx4_linear(&a, s);
+        return mx4_linear(&a, mx4_plan_one_chain, s);
     };
     if (int rc = seam(nullptr, m->blocks[0].n1w, m->blocks[0].n1b, h, UITK_T_MX4)) return rc;
     for (int b = 0; b < g.depth; ++b) {

@@ -126,7 +126,7 @@ struct Mx4LinearArgs {
     const void* residual; int64_t ldr;                                      // of the output's type, added last
     void* out; int64_t ldo; int out_type;                                   // MT_MX4: out = codes, out_scales its scales
     char* out_scales; int64_t out_S;
-    unsigned ngroups;                                                       // column groups of the rows kernel
+    unsigned ngroups; int chains;                                           // rows kernel: column groups; waves that share K (not more than its records)
 };
 
 __device__ __forceinline__ mx_f4 mx4_bias4(const Mx4LinearArgs& a, int64_t n) {
@@ -222,10 +222,10 @@ __device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, in
     else mx4_finish4<MT_BF16>(a.out, m * a.ldo + n, a.residual, m * a.ldr + n, in, v);
 }
 
-// ---- few rows, or few tiles: latency.  A workgroup computes 32 NT outputs (n) x 32 tokens (m); its NW waves take the records of K in turn, each
-// with its own accumulators, and join them through LDS in a fixed order.  Operands go from memory to registers in fragment order, a
-// record of weights ahead of its product; activations that are not packed yet are quantised by the lane that multiplies them (lane l of
-// the B operand owns row l % 32, block l / 32: a whole block).  Bound by reading the weights where there are many (13 x 8192 x 8192, packed x:
+// ---- few rows, or few tiles: latency.  A workgroup computes 32 NT outputs (n) x 32 tokens (m); its NW waves (or the first of them alone: a.chains)
+// take the records of K in turn, each with its own accumulators, and join them through LDS in a fixed order.  Operands go from memory to
+// registers in fragment order, a record of weights ahead of its product; activations that are not packed yet are quantised by the lane that
+// multiplies them (lane l of the B operand owns row l % 32, block l / 32: a whole block).  Bound by reading the weights where there are many (13 x 8192 x 8192, packed x:
 // 11.9 us, 3.0 TB/s of weights), by the latency of a launch and one trip to memory where there are few (1 x 2304 x 768: 3.2 us).
 template <typename XT>
 __device__ __forceinline__ Mx4Block mx4_x_fragment(const Mx4LinearArgs& a, int64_t row, int64_t k) {
@@ -260,14 +260,14 @@ __global__ void __launch_bounds__(64 * NW) mx4_rows_kernel(Mx4LinearArgs a) {
         for (int f = 0; f < NT * 2; ++f) wf[f] = *(const mx_i4*)(wc + f * 1024);
         ws = *(const int*)(a.w_scales + rec * MX4_SCALES + lane * 4) >> (16 * half);
     };
-    if (ng * MX4_ROWS + 32 * half < a.N && wave < a.S) {                    // (an out_type of 4 bits pads its columns to 128: such a group multiplies nothing)
+    if (ng * MX4_ROWS + 32 * half < a.N && wave < a.chains) {               // (an out_type of 4 bits pads its columns to 128: such a group multiplies nothing)
         weights(wave);
-        for (int64_t s = wave; s < a.S; s += NW) {
+        for (int64_t s = wave; s < a.S; s += a.chains) {
             mx_i4 w[NT * 2];
 #pragma unroll
             for (int f = 0; f < NT * 2; ++f) w[f] = wf[f];
             const int wsc = ws;
-            if (s + NW < a.S) weights(s + NW);
+            if (s + a.chains < a.S) weights(s + a.chains);
             Mx4Block x0, x1;                                                // the two halves of the record; their scales in bytes 0 and 1 where packed
             if constexpr (PACKED) {
                 const int64_t rec = (m0 >> 6) * a.S + s;
@@ -292,12 +292,11 @@ __global__ void __launch_bounds__(64 * NW) mx4_rows_kernel(Mx4LinearArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) *(mx_f4*)&mine[c * LDT + 32 * rt + 8 * q + 4 * g] = mx_f4{acc[rt][4 * q], acc[rt][4 * q + 1], acc[rt][4 * q + 2], acc[rt][4 * q + 3]};
     __syncthreads();
-    const int nw = (int)min((int64_t)NW, a.S);                              // (the other waves had no record)
     for (int i = threadIdx.x; i < 32 * 8 * NT; i += 64 * NW) {              // (whole waves: the 4-bit store exchanges maxima between lanes)
         const int t = i / (8 * NT), n4 = i % (8 * NT) * 4;
         const float* p = red + t * LDT + n4;
         mx_f4 s = *(const mx_f4*)p;
-        for (int w = 1; w < nw; ++w) s += *(const mx_f4*)(p + w * 32 * LDT);
+        for (int w = 1; w < a.chains; ++w) s += *(const mx_f4*)(p + w * 32 * LDT);
         float v[4] = {s[0], s[1], s[2], s[3]};
         const int64_t n = nt * 32 * NT + n4;
         mx4_store4(a, m0 + t, n, mx4_bias4(a, n), v);
@@ -593,11 +592,12 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static bool on_element(const void* p, int type) { return (uintptr_t)p % (type == UITK_T_F32 ? 4 : 2) == 0; }
 
 template <int NT, int NW>
-static hipError_t mx4_launch_rows(Mx4LinearArgs& a, hipStream_t s) {
+static hipError_t mx4_launch_rows(Mx4LinearArgs& a, bool one_chain, hipStream_t s) {
     const int64_t cols = a.out_type == MT_MX4 ? a.out_S * MX4_K : a.N;
     const int64_t ngroups = (cols + 32 * NT - 1) / (32 * NT), mt = (a.M + 31) / 32;
     if (mt * ngroups > ((int64_t)1 << 32) / (64 * NW) - 1) return hipErrorInvalidConfiguration;
     a.ngroups = (unsigned)ngroups;
+    a.chains = one_chain ? 1 : (int)std::min<int64_t>(NW, a.S);
     const dim3 grid((unsigned)(mt * ngroups));
     constexpr int lds = NW * 32 * (32 * NT + 4) * 4;
     auto go = [&](auto kernel) {
@@ -690,7 +690,11 @@ int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type) {
     return mx4_plan(M, N, K, x_type == UITK_T_MX4).quantize_first ? mx4_bytes(M, K) : 0;
 }
 
-int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
+int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) { return mx4_linear(u, mx4_plan, stream); }
+
+}  // extern "C"
+
+int uitk::mx4_linear(const uitk_mx4_linear_args* u, Mx4Plan (*rule)(int64_t, int64_t, int64_t, bool), void* stream) {
     if (!u) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: null arguments");
     if (int rc = mx4_check_matrix("uitk_mx4_linear (x)", u->M, u->K)) return rc;
     if (u->N < 1 || u->N > MX4_MAX_K) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: N must be 1 .. 2^20");
@@ -718,7 +722,7 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     a.out = u->out; a.ldo = u->ldo; a.out_type = u->out_type;
     if (u->out_type == UITK_T_MX4) { a.out_S = (u->N + MX4_K - 1) / MX4_K; a.out_scales = (char*)u->out + mx4_records(u->M, u->N) * MX4_CODES; }
     hipStream_t s = (hipStream_t)stream;
-    const Mx4Plan plan = mx4_plan(u->M, u->N, u->K, u->x_type == UITK_T_MX4);
+    const Mx4Plan plan = rule(u->M, u->N, u->K, u->x_type == UITK_T_MX4);
     if (plan.quantize_first) {
         if (!u->workspace || !aligned16(u->workspace)) return set_error(UITK_ERR_INVALID_ARG, "uitk_mx4_linear: needs a 16-byte aligned workspace (uitk_mx4_linear_workspace)");
         if (int rc = uitk_mx4_quantize(u->x, u->x_type, u->M, u->K, u->ldx, u->workspace, stream)) return rc;
@@ -726,12 +730,10 @@ int uitk_mx4_linear(const uitk_mx4_linear_args* u, void* stream) {
     }
     const hipError_t e = plan.kernel == MX4_TILE256   ? mx4_launch_tile<256, 128, 2, 2>(a, s)
                          : plan.kernel == MX4_TILE128 ? mx4_launch_tile<128, 128, 2, 2>(a, s)
-                         : plan.kernel == MX4_ROWS64  ? mx4_launch_rows<2, 8>(a, s)
-                         : plan.kernel == MX4_ROWS16  ? mx4_launch_rows<1, 16>(a, s)
-                                                      : mx4_launch_rows<1, 8>(a, s);
+                         : plan.kernel == MX4_ROWS64  ? mx4_launch_rows<2, 8>(a, plan.one_chain, s)
+                         : plan.kernel == MX4_ROWS16  ? mx4_launch_rows<1, 16>(a, plan.one_chain, s)
+                                                      : mx4_launch_rows<1, 8>(a, plan.one_chain, s);
     if (e == hipErrorInvalidConfiguration) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_linear: more outputs than one launch takes");
     MX4_HIP(e);
     return UITK_OK;
 }
-
-}  // extern "C"

@@ -4,9 +4,10 @@
                      +-{0, .5, 1, 1.5, 2, 3, 4, 6} times it: 4.25 bits an element.  A block holding an infinity or a NaN is NaN as a whole.
 `Mx4Tensor.dequantize()`  the values the codes stand for
 `linear(x, w)`     = residual + act(Q(x) @ W.T + bias) on the 4-bit matrix pipe; the sums are fp32, the output is rounded once.  `x` a tensor
-                     (rounded to 4 bits on the way in) or an `Mx4Tensor`; `w` an `Mx4Tensor`, made once from the weights with `quantize`
+                     (rounded to 4 bits on the way in) or an `Mx4Tensor`; `w` an `Mx4Tensor`, made once from the weights with `quantize`.
+                     The same call gives the same bits; a row among a different number of rows may be added in another order (fp32 rounding)
 
-What `UITBase(precision='mx4')` runs its dense layers on (uit_mobile_amd/models/uit.py).  CUDA tensors only, on the tensors' device and its
+What `UITBase(precision='mx4')` runs its dense layers on (uit_mobile_amd/models/uit.py), there in one order whatever the batch.  CUDA tensors only, on the tensors' device and its
 current stream; enqueue-only, safe inside a HIP graph capture.  No gradients: like the rest of this package these are inference operators,
 and a call that autograd would have to record is refused.
 """
