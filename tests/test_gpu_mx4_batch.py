@@ -55,3 +55,23 @@ def test_a_clip_does_not_see_the_batch_it_is_in(name):
         for lo, hi in ((0, 1), (5, 6), (0, 3), (7, 16), (0, B // 2), (B // 2, B), (1, B)):
             got = m(x[lo:hi], amax_sync=lambda slots: slots.copy_(top[0].expand(64)))
             assert torch.equal(got, want[lo:hi]), (name, lo, hi, float((got - want[lo:hi]).abs().max()))
+
+
+@pytest.mark.parametrize("T,crops,copies", [(160000, 1, 44), (320000, 2, 22)])
+def test_every_clip_of_every_chunk_is_that_clip_alone(T, crops, copies):
+    """More rows (a clip's crop each) than the engine's 3 GiB workspace takes at once: 704 of the default width in two chunks, the second
+    one short, their border inside a copy of the clips and inside a clip's crops.  Sixteen clips many times over: every copy has the bits of
+    the sixteen by themselves."""
+    m = uneven(build(dim=768, heads=12, depth=2, mlp_ratio=4.0, tl=1012)).cuda().eval()
+    tokens = 4 * ((1012 if crops > 1 else m.num_frames(T)) // 16)
+    floats = 16 * 16 + 2 * 768 + 3 * 768 + 768                             # fp32 work buffers of a token
+    per_chunk = (3 << 30) // (tokens * floats * 4)
+    rows = 16 * crops * copies
+    assert m.num_crops(T) == crops and per_chunk < rows < 2 * per_chunk and per_chunk % (16 * crops) and (crops == 1 or per_chunk % crops)
+    few = torch.from_numpy(synth_pcm_i16(16, T, seed=2)).cuda()
+    with torch.no_grad():
+        want, want_logits = m(few, return_logits=True)
+        got, got_logits = m(few.repeat(copies, 1), return_logits=True)
+    assert torch.isfinite(want).all()
+    assert torch.equal(got.view(copies, 16, -1), want.expand(copies, 16, -1))
+    assert torch.equal(got_logits.reshape(copies, 16, -1), want_logits.reshape(1, 16, -1).expand(copies, 16, -1))
