@@ -371,8 +371,9 @@ class UITBase(nn.Module):
 
     def _not_general(self, what):
         if self.general:
-            raise NotImplementedError(f"{what} belongs to the MFMA kernels (the published factories' geometry); this model runs on the general "
-                                      "fp32 engine, which rounds nothing, calibrates nothing and has no options")
+            raise NotImplementedError(f"{what} belongs to the MFMA kernels (the published factories' geometry); this model runs on the general " +
+                                      ("engine with its dense layers rounded to 4 bits, which calibrates nothing and has no options" if self.precision == 'mx4' else
+                                       "fp32 engine, which rounds nothing, calibrates nothing and has no options"))
 
     def _config(self, precision=None):
         return _lib.Config(depth=self.depth, embed_dim=self.embed_dim, num_heads=self.num_heads,
@@ -544,8 +545,12 @@ class UITBase(nn.Module):
         if self.general and not self._warned_general:
             self._warned_general = True
             warnings.warn("uit_mobile_amd: this configuration is outside the geometry of the published factories (embed 128, 2 heads, MLP x 3, 64 mels, "
-                          "n_fft 512, 16 x 16 patches, 6 time patches): it runs on the library's GENERAL fp32 engine -- on the device, in the reference's "
-                          "order of operations, an order of magnitude slower than the MFMA kernels", UitkSetupWarning, stacklevel=4)
+                          "n_fft 512, 16 x 16 patches, 6 time patches): " +
+                          ("precision='mx4' runs on the library's GENERAL engine with the weights and activations of its blocks' dense layers rounded to 4 bits "
+                           "-- a throughput mode, outside the parity budget (synthetic weights: logits off by 0.13 to 0.40 rms and up to 1.5, where they "
+                           "spread by 1.9 to 2.7 over the classes); precision 'f32' rounds nothing" if self.precision == 'mx4' else
+                           "it runs on the library's GENERAL fp32 engine -- on the device, in the reference's "
+                           "order of operations, an order of magnitude slower than the MFMA kernels"), UitkSetupWarning, stacklevel=4)
         if self.precision in _CALIBRATING and _from_forward and not self._warned_setup:
             self._warned_setup = True
             warnings.warn("uit_mobile_amd: this forward call builds the parameter image first (weight calibration + acceptance check, "
