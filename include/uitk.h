@@ -382,7 +382,7 @@ typedef struct uitk_mx4_linear_args {
     void* workspace;       /* uitk_mx4_linear_workspace bytes, 16-byte aligned, of this call until it has run (NULL when 0) */
     int64_t M, N, K, ldx, ldr, ldo;
     int32_t x_type, out_type; /* uitk_type */
-    int32_t act;           /* 0 none, 1 ReLU, 2 exact (erf) GELU */
+    int32_t act;           /* 0 none, 1 ReLU, 2 GELU: x Phi(x), off by less than 2^-21 max(1, |y|) (absolute: below x = -4 that is no longer small beside y) */
     int32_t reserved;      /* 0 */
 } uitk_mx4_linear_args;
 int64_t uitk_mx4_linear_workspace(int64_t M, int64_t N, int64_t K, int x_type);   /* bytes; -1: out of range */

@@ -122,7 +122,7 @@ struct Mx4LinearArgs {
     const char* w; const char* w_scales;                                    // packed [N, K]
     int64_t N, S;                                                           // S = records along K
     const float* bias;
-    int act;                                                                // 0 none, 1 ReLU, 2 exact GELU
+    int act;                                                                // 0 none, 1 ReLU, 2 GELU (mx4_gelu)
     const void* residual; int64_t ldr;                                      // of the output's type, added last
     void* out; int64_t ldo; int out_type;                                   // MT_MX4: out = codes, out_scales its scales
     char* out_scales; int64_t out_S;

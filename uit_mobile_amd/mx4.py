@@ -173,8 +173,8 @@ def quantize(x):
 
 
 def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
-    """residual + act(Q(x) @ w.T + bias): x [..., K] tensor or Mx4Tensor, w Mx4Tensor [N, K], bias [N], act None / 'relu' / 'gelu' (exact),
-    residual [..., N] of the output's type -> [..., N].
+    """residual + act(Q(x) @ w.T + bias): x [..., K] tensor or Mx4Tensor, w Mx4Tensor [N, K], bias [N], act None / 'relu' / 'gelu' (x Phi(x), by
+    a fitted polynomial: off by less than 2^-21 max(1, |y|)), residual [..., N] of the output's type -> [..., N].
 
     out_dtype: float32 / float16 / bfloat16 (default: x's type, or the residual's; float32 for a packed x), or 'mx4': the output is an
     Mx4Tensor, the next layer's x (no residual then).  out: write there instead (a contiguous tensor of the output's shape and type;
