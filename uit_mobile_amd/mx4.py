@@ -57,12 +57,13 @@ def check_tensor(t, name):
 
 def as_rows(t, K):
     """[..., K] -> (a tensor that holds its rows, their distance in elements): `t` itself where its strides allow, else a copy."""
-    if t.is_contiguous():
+    if K > 1 and t.is_contiguous():
         return t, K
     rows = t.numel() // K if K else 0
     v = t.reshape(rows, K)
     if K > 1 and v.stride(1) != 1 or rows > 1 and v.stride(0) < K:
         v = v.contiguous()
+    v = v.resolve_neg()                                                     # (imag of a conjugate: rows of one element reach this without a copy)
     return v, (v.stride(0) if rows > 1 else K)
 
 
@@ -88,7 +89,7 @@ def check_vector(t, name, n, device, keep):
     """A per-channel parameter: [n] on `device` -> the address of its values in float32 (0: None).  What had to be converted joins `keep`."""
     if t is None:
         return 0
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device.index and t.dim() == 1 and t.numel() == n
+    if (n > 1 and isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device.index and t.dim() == 1 and t.numel() == n
             and t.is_contiguous() and not (t.requires_grad and torch.is_grad_enabled())):
         return t.data_ptr()
     check_tensor(t, name)
@@ -96,7 +97,7 @@ def check_vector(t, name, n, device, keep):
         raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    keep.append(t.to(torch.float32).contiguous())
+    keep.append(t.to(torch.float32).resolve_neg().contiguous())
     return keep[-1].data_ptr()
 
 
@@ -216,7 +217,7 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
     if out is not None:
         if to_mx4:
             raise ValueError("out is not supported for a 4-bit output")
-        if out.shape != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous():
+        if out.shape != shape or out.dtype != out_dtype or out.device != device or not out.is_contiguous() or out.is_neg():
             raise ValueError(f"out must be a contiguous {tuple(shape)} {out_dtype} on {device}")
         mine = span(out)
         for name, t in (("x", x.data if packed else x), ("w", w.data), ("bias", bias)):
