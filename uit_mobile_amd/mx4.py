@@ -41,6 +41,11 @@ def run(fn, device, *args):
         _lib.check(rc, fn.__name__)
 
 
+# The caller's tensor has new contents: its version counter says so, as after any in-place operation -- a backward pass that saved the old contents
+# refuses, and a model whose parameter it is packs its weights again.
+written = torch.autograd.graph.increment_version
+
+
 def check_tensor(t, name):
     """A CUDA tensor of a type these operators take that needs no gradient -> its uitk_type (shared with norms.py)."""
     if not isinstance(t, torch.Tensor):
@@ -239,4 +244,6 @@ def linear(x, w, bias=None, act=None, residual=None, out_dtype=None, out=None):
     args = _LINEAR_ARGS.pack(src.data_ptr(), w.data.data_ptr(), b, 0 if res is None else res.data_ptr(), dst.data_ptr(), 0 if ws is None else ws.data_ptr(),
                              M, N, K, ldx, ldr, N, x_type, out_type, _ACTS[act], 0)
     run(_lib.packed("uitk_mx4_linear"), device, args)
+    if out is not None:
+        written(out)
     return result

@@ -13,7 +13,7 @@ import struct
 import torch
 
 from . import _lib
-from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, new, overlaps, run, span
+from .mx4 import _TYPES, Mx4Tensor, as_rows, check_tensor, check_vector, new, overlaps, run, span, written
 
 _ARGS = struct.Struct("10Q7q8if4x")                                          # uitk_block_norm_args
 _KINDS = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
@@ -106,4 +106,6 @@ def block_norm(y, residual, *, post=None, gate=None, scale=None, pre=None, kind=
     args = _ARGS.pack(0 if yv is None else yv.data_ptr(), r.data_ptr(), 0 if ro is None else ro.data_ptr(), h_ptr, g, s, post_w, post_b, pre_w, pre_b,
                       rows, ldy, ldr, ldro, D, ldg, gate_rows, D, y_type, r_type, h_type, gate_type, _KINDS[kind], post is not None, pre is not None, eps)
     run(_lib.packed("uitk_block_norm"), device, args)
+    if inplace and ro is not None:
+        written(residual)
     return r_out, h
