@@ -1,7 +1,7 @@
 """GPU: a few forwards of the `f32` rung (UiT-XS x 8192 clips) and of one general-engine geometry, for a rocprofv3 --kernel-trace --stats
-breakdown of the plain fp32 path (which kernel the time goes to):
+breakdown of the plain fp32 path (which kernel the time goes to), or of the default UITBase in f32 / mx4 ("default" / "default_mx4"):
 
-    rocprofv3 --kernel-trace --stats -d gpurun_out/f32prof -o f32 -- python3 tools/f32_breakdown.py"""
+    rocprofv3 --kernel-trace --stats -d gpurun_out/f32prof -o f32 -- python3 tools/f32_breakdown.py [default_mx4]"""
 import sys
 import warnings
 from pathlib import Path
@@ -21,8 +21,8 @@ if which == "f32":
     m = models.uit_xs(outputdim=537, target_length=102, precision="f32")
     m.load_state_dict({k: torch.from_numpy(np.asarray(v)) for k, v in make_state_dict("uit_xs", 3).items()})
     B, T = 8192, 16000
-elif which == "default":
-    m = models.UITBase(outputdim=527)                  # the constructor's own defaults: 768 wide, 12 blocks, 12 heads, 85.7 M parameters
+elif which in ("default", "default_mx4"):              # the constructor's own defaults: 768 wide, 12 blocks, 12 heads, 85.7 M parameters
+    m = models.UITBase(outputdim=527, precision="mx4" if which == "default_mx4" else None)
     B, T = 64, 160000
 else:
     m = models.UITBase(embed_dim=128, depth=12, num_heads=2, mlp_ratio=3.0, pooling="mean", attention_type="BNeckAttention", act_layer=nn.ReLU,

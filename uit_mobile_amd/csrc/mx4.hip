@@ -226,7 +226,8 @@ __device__ __forceinline__ void mx4_store4(const Mx4LinearArgs& a, int64_t m, in
 // take the records of K in turn, each with its own accumulators, and join them through LDS in a fixed order.  Operands go from memory to
 // registers in fragment order, a record of weights ahead of its product; activations that are not packed yet are quantised by the lane that
 // multiplies them (lane l of the B operand owns row l % 32, block l / 32: a whole block).  Bound by reading the weights where there are many (13 x 8192 x 8192, packed x:
-// 11.9 us, 3.0 TB/s of weights), by the latency of a launch and one trip to memory where there are few (1 x 2304 x 768: 3.2 us).
+// 10.8 us, 3.3 TB/s of weights; 13 x 8192 x 8320: 8.1 us, 4.5 TB/s -- rows of records a power of two apart are read in step, likely from few
+// channels), by the latency of a launch and one trip to memory where there are few (1 x 2304 x 768: 3.1 us).
 template <typename XT>
 __device__ __forceinline__ Mx4Block mx4_x_fragment(const Mx4LinearArgs& a, int64_t row, int64_t k) {
     Mx4Block b{mx_i4{0, 0, 0, 0}, 0};
@@ -309,8 +310,8 @@ __global__ void __launch_bounds__(64 * NW) mx4_rows_kernel(Mx4LinearArgs a) {
 // its way while s is multiplied, s + 2 follows into the slot of s once the second half of s is in registers.  One barrier per stage,
 // between the two halves, and every load issued behind a product, so that the matrix pipe has work throughout.  (A third slot costs a
 // workgroup per CU and is slower: 16128 x 2304 x 768, 128 x 128 tile, 3 / 2 slots 32.5 / 28.7 us; 8192^3, 256 x 128: 265 / 262; loads behind products instead of in one go: 254.)
-// 8192^3: 4.3 PFLOP/s at 1.7 GHz and 53 % matrix-pipe occupancy: the card is at its power limit (products from registers alone, on the same
-// random operands: 6.3 PFLOP/s at 1.55 GHz; on zeros 9.7 at 2.4).  Narrow K: bound by writing the output (16128 x 2304 x 768: 81 MB, 2.9 TB/s).
+// 8192^3: 4.3 PFLOP/s at 1.7 GHz, the matrix pipe busy in 56 % of the cycles.  The clock is the card's power limit; the pipe's idle time is not: products
+// alone, on random operands, reach 6.2 PFLOP/s from registers (95 % busy, 1.55 GHz) and 5.7 from LDS (81 %, 1.68 GHz).  Narrow K: bound by writing the output (16128 x 2304 x 768: 81 MB, 2.9 TB/s).
 __device__ __forceinline__ void mx4_dma16(unsigned lds, unsigned off, const char* src) {       // 64 lanes x 16 B -> 1 KB at lds
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(src) : "memory", "m0");
 }
@@ -650,7 +651,9 @@ int uitk_mx4_quantize(const void* x, int type, int64_t rows, int64_t K, int64_t 
     char* codes = (char*)q;
     char* scales = codes + R * S * MX4_CODES;
     if ((R * S + 3) / 4 > MX4_MAX_GRID) return set_error(UITK_ERR_UNSUPPORTED, "uitk_mx4_quantize: more elements than one launch takes");
-    const bool split = R * S <= 1024;                                       // (1021 x 1000 f16, a record to a workgroup / to a wave: 3.5 / 6.8 us)
+    // a record to a workgroup / to a wave, us: bf16 1021 x 1000 (128 records) 3.4 / 6.8, 2048 x 4096 (1024) 4.1 / 4.8, 8192 x 4096 (4096) 13.6 / 17.1; fp32
+    // 1021 x 1000 3.4 / 7.2, 16128 x 768 (1512) 9.8 / 9.7
+    const bool split = R * S <= 1024;
     const dim3 grid((unsigned)(split ? R * S : (R * S + 3) / 4)), block(256);
     hipStream_t s = (hipStream_t)stream;
     auto launch = [&](auto kernel, const auto* p) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p, rows, K, ld, R, S, codes, scales); };
