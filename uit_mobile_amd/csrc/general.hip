@@ -621,19 +621,26 @@ static int gen_reserve(uitk_general* m, int64_t B, int64_t T, hipStream_t s) {
     if (int rc = gen_check_shape(m, B, T)) return rc;
     const int nF = gen_num_frames(m, T), nc = gen_num_crops(m, T), nt = gen_time_patches(m, T);
     const int ntok = m->g.GF * nt + m->g.cls;
-    if (int rc = gen_grow(&m->frames, &m->frames_cap, (size_t)B * nF * m->g.M * 4, s)) return rc;
+    const size_t had_frames = m->frames_cap, had_work = m->work_cap, had_probs = m->rowprobs_cap;
+    int rc = gen_grow(&m->frames, &m->frames_cap, (size_t)B * nF * m->g.M * 4, s);
+    if (m->frames_cap != had_frames) m->fe_B = m->fe_T = 0;                // (what a front-end call left in the old buffer is gone)
+    if (rc) return rc;
     const int64_t rows = B * nc;
     const size_t per_row = gen_row_floats(m->g, ntok, m->mx4()) * 4;
     int64_t chunk = (int64_t)std::max<size_t>(1, GEN_WORK_BYTES / per_row);
     chunk = std::min<int64_t>(chunk, rows);
     chunk = std::min<int64_t>(chunk, (int64_t)65535 * 64 / ntok);          // the dense kernel's grid: 64 token rows per workgroup in gridDim.y
     if (chunk < 1) return set_error(UITK_ERR_UNSUPPORTED, "general engine: one clip-crop exceeds the work buffer");
-    if (int rc = gen_grow(&m->work, &m->work_cap, (size_t)chunk * per_row, s)) return rc;
+    rc = gen_grow(&m->work, &m->work_cap, (size_t)chunk * per_row, s);
+    if (m->work_cap != had_work) m->work_rows = 0;                         // (until every buffer is there: a failed growth leaves none behind)
+    if (rc) return rc;
     // (work_rows below can exceed this call's chunk where an earlier shape grew the buffer; the packed operands follow it)
     if (m->mx4())
-        if (int rc = gen_grow(&m->work4, &m->work4_cap, gen_work4(m->g, std::min<int64_t>((int64_t)(m->work_cap / per_row), rows) * ntok).bytes, s)) return rc;
+        if ((rc = gen_grow(&m->work4, &m->work4_cap, gen_work4(m->g, std::min<int64_t>((int64_t)(m->work_cap / per_row), rows) * ntok).bytes, s))) return rc;
+    rc = gen_grow(&m->rowprobs, &m->rowprobs_cap, nc > 1 ? (size_t)rows * m->g.C * 4 : 0, s);
+    if (m->rowprobs_cap < had_probs) m->work_rows = 0;
+    if (rc) return rc;
     m->work_rows = (int64_t)(m->work_cap / per_row); m->work_ntok = ntok;
-    if (int rc = gen_grow(&m->rowprobs, &m->rowprobs_cap, nc > 1 ? (size_t)rows * m->g.C * 4 : 0, s)) return rc;
     return UITK_OK;
 }
 
