@@ -337,7 +337,8 @@ int uitk_kws_transform(float* y_pred, const float* y, int64_t B, int32_t C, int3
  * fc1_w [mlp_hidden, embed], fc2_w [embed, mlp_hidden], head_w [outputdim, embed], mel_fb [n_fft / 2 + 1, n_mels], window [win_size].
  * Limits: n_fft even, 16..4096 (a power of two runs an FFT; any other value, up to 2048, the DFT sum in double); patch_size a multiple of 4;
  * embed_dim, mlp_hidden and the attention's inner width multiples of 16.
- * Same calling rules as the uitk_model functions: one handle per device, enqueue-only on `stream` once the workspace is reserved,
+ * Same calling rules as the uitk_model functions: one handle per device, enqueue-only on `stream` once the workspace is reserved
+ * (a call recorded into a graph keeps its buffers until the handle is destroyed: larger shapes may run between replays, the handle must outlive them),
  * uitk_general_frontend / uitk_general_encode are the two stages of uitk_general_forward (the batch amax -- uitk_general_amax_ptr,
  * UITK_AMAX_SLOTS floats -- may be MAX-reduced across ranks between them), errors through uitk_last_error.
  * Stand in for: UITBase(**kwargs) + load_state_dict + .to(DEVICE).eval() and model(x) (models/uit.py:253-363, 452-493). */

@@ -39,3 +39,23 @@ def test_a_growth_that_a_capture_refuses_leaves_the_state_good(precision):
                     m(more)
         torch.cuda.synchronize()
         assert torch.equal(m.encode(state), want)
+
+
+@pytest.mark.parametrize("precision", ["f32", "mx4"])
+@pytest.mark.parametrize("T", [16000, 40000])                                # one crop, three crops
+def test_a_graph_keeps_its_buffers_when_a_larger_batch_grows_them(precision, T):
+    m = build(precision=precision).cuda().eval()
+    m.prepare("cuda", (4, T), dtype=torch.int16)
+    x, more = (torch.from_numpy(synth_pcm_i16(n, T, seed=5)).cuda() for n in (4, 200))
+    with torch.no_grad():
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m(x)
+        for i in range(3):
+            big = m(more[:100 * (i + 1) if i < 2 else 200])                  # grows, grows again, stays
+            keep = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(4)]     # what a freed buffer would be given to
+            x.copy_(torch.from_numpy(synth_pcm_i16(4, T, seed=30 + i)))
+            g.replay()
+            got = out.clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, m(x)) and torch.isfinite(big).all() and len(keep) == 4

@@ -402,6 +402,8 @@ struct uitk_general {
     std::vector<size_t> packed_off;          // ... [4 b + layer] -> bytes into `packed`
     float* work4 = nullptr; size_t work4_cap = 0;      // precision 'mx4': the packed operands of the chunk (gen_work4)
     int64_t fe_B = 0, fe_T = 0;
+    bool captured = false;                   // a call of this handle was recorded into a graph: buffers that grow are ...
+    std::vector<void*> kept;                 // ... replaced, and the old ones live as long as the handle
     bool mx4() const { return cfg.precision == UITK_PREC_MX4; }
 };
 
@@ -478,14 +480,23 @@ static GenWork4 gen_work4(const GenGeom& g, int64_t M) {
 }
 constexpr size_t GEN_WORK_BYTES = (size_t)3 << 30;                        // rows are processed in chunks that fit this
 
-static int gen_grow(float** p, size_t* cap, size_t bytes, hipStream_t s) {
+// (nothing can be recorded on the null stream)
+static void gen_note_capture(uitk_general* m, hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (m->captured || s == nullptr) return;
+    if (hipStreamIsCapturing(s, &status) != hipSuccess) (void)hipGetLastError();
+    else m->captured = status != hipStreamCaptureStatusNone;
+}
+
+static int gen_grow(uitk_general* m, float** p, size_t* cap, size_t bytes, hipStream_t s) {
     if (bytes <= *cap) return UITK_OK;
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;          // growing synchronises: never inside a stream capture
     if (hipStreamIsCapturing(s, &capturing) != hipSuccess) (void)hipGetLastError();
     else if (capturing != hipStreamCaptureStatusNone)
         return set_error(UITK_ERR_WORKSPACE, "general engine: the workspace has to grow for this shape and the stream is being captured (uitk_general_reserve first)");
     GEN_HIP(hipDeviceSynchronize());                                       // (the device may still be reading the old buffer)
-    if (*p) (void)hipFree(*p);
+    if (*p && m->captured) m->kept.push_back(*p);                          // (a graph that is replayed later uses it)
+    else if (*p) (void)hipFree(*p);
     *p = nullptr; *cap = 0;
     GEN_HIP(hipMalloc((void**)p, bytes));
     *cap = bytes;
@@ -609,6 +620,7 @@ int uitk_general_destroy(uitk_general* m) {
     if (m->rowprobs) (void)hipFree(m->rowprobs);
     if (m->packed) (void)hipFree(m->packed);
     if (m->work4) (void)hipFree(m->work4);
+    for (void* p : m->kept) (void)hipFree(p);
     delete m;
     return UITK_OK;
 }
@@ -622,7 +634,7 @@ static int gen_reserve(uitk_general* m, int64_t B, int64_t T, hipStream_t s) {
     const int nF = gen_num_frames(m, T), nc = gen_num_crops(m, T), nt = gen_time_patches(m, T);
     const int ntok = m->g.GF * nt + m->g.cls;
     const size_t had_frames = m->frames_cap, had_work = m->work_cap, had_probs = m->rowprobs_cap;
-    int rc = gen_grow(&m->frames, &m->frames_cap, (size_t)B * nF * m->g.M * 4, s);
+    int rc = gen_grow(m, &m->frames, &m->frames_cap, (size_t)B * nF * m->g.M * 4, s);
     if (m->frames_cap != had_frames) m->fe_B = m->fe_T = 0;                // (what a front-end call left in the old buffer is gone)
     if (rc) return rc;
     const int64_t rows = B * nc;
@@ -631,13 +643,13 @@ static int gen_reserve(uitk_general* m, int64_t B, int64_t T, hipStream_t s) {
     chunk = std::min<int64_t>(chunk, rows);
     chunk = std::min<int64_t>(chunk, (int64_t)65535 * 64 / ntok);          // the dense kernel's grid: 64 token rows per workgroup in gridDim.y
     if (chunk < 1) return set_error(UITK_ERR_UNSUPPORTED, "general engine: one clip-crop exceeds the work buffer");
-    rc = gen_grow(&m->work, &m->work_cap, (size_t)chunk * per_row, s);
+    rc = gen_grow(m, &m->work, &m->work_cap, (size_t)chunk * per_row, s);
     if (m->work_cap != had_work) m->work_rows = 0;                         // (until every buffer is there: a failed growth leaves none behind)
     if (rc) return rc;
     // (work_rows below can exceed this call's chunk where an earlier shape grew the buffer; the packed operands follow it)
     if (m->mx4())
-        if ((rc = gen_grow(&m->work4, &m->work4_cap, gen_work4(m->g, std::min<int64_t>((int64_t)(m->work_cap / per_row), rows) * ntok).bytes, s))) return rc;
-    rc = gen_grow(&m->rowprobs, &m->rowprobs_cap, nc > 1 ? (size_t)rows * m->g.C * 4 : 0, s);
+        if ((rc = gen_grow(m, &m->work4, &m->work4_cap, gen_work4(m->g, std::min<int64_t>((int64_t)(m->work_cap / per_row), rows) * ntok).bytes, s))) return rc;
+    rc = gen_grow(m, &m->rowprobs, &m->rowprobs_cap, nc > 1 ? (size_t)rows * m->g.C * 4 : 0, s);
     if (m->rowprobs_cap < had_probs) m->work_rows = 0;
     if (rc) return rc;
     m->work_rows = (int64_t)(m->work_cap / per_row); m->work_ntok = ntok;
@@ -664,6 +676,7 @@ int uitk_general_frontend(uitk_general* m, const void* pcm, int in_dtype, int64_
     if (int rc = gen_check_shape(m, B, T)) return rc;
     if (!pcm) return set_error(UITK_ERR_INVALID_ARG, "null pcm");
     if (in_dtype != UITK_IN_F32 && in_dtype != UITK_IN_I16) return set_error(UITK_ERR_INVALID_ARG, "unknown in_dtype");
+    gen_note_capture(m, (hipStream_t)stream);
     if (int rc = gen_reserve(m, B, T, (hipStream_t)stream)) return rc;
     if (int rc = gen_run_frontend(m, pcm, in_dtype, B, T, (hipStream_t)stream)) return rc;
     m->fe_B = B; m->fe_T = T;
@@ -726,6 +739,7 @@ int uitk_general_encode(uitk_general* m, int64_t B, int64_t T, float* probs, flo
     if (m->fe_B != B || m->fe_T != T) return set_error(UITK_ERR_INVALID_ARG, "uitk_general_encode: no front-end output of this shape (uitk_general_frontend first)");
     if (logits && m->g.pooling == 1) return set_error(UITK_ERR_INVALID_ARG, "pooling 'dm' has no pre-sigmoid output");
     hipStream_t s = (hipStream_t)stream;
+    gen_note_capture(m, s);
     GenGeom g = m->g;
     const int nF = gen_num_frames(m, T), nc = gen_num_crops(m, T);
     g.nt = gen_time_patches(m, T); g.np = g.GF * g.nt; g.ntok = g.np + g.cls;
