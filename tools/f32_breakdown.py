@@ -1,7 +1,7 @@
 """GPU: a few forwards of the `f32` rung (UiT-XS x 8192 clips) and of one general-engine geometry, for a rocprofv3 --kernel-trace --stats
 breakdown of the plain fp32 path (which kernel the time goes to), or of the default UITBase in f32 / mx4 ("default" / "default_mx4"):
 
-    rocprofv3 --kernel-trace --stats -d gpurun_out/f32prof -o f32 -- python3 tools/f32_breakdown.py [default_mx4]"""
+    rocprofv3 --kernel-trace --stats -d DIR -o f32 -- python3 tools/f32_breakdown.py [default_mx4]"""
 import sys
 import warnings
 from pathlib import Path
